@@ -236,6 +236,67 @@ struct PrefillArgs {
 };
 cudaError_t launch_paged_prefill(const PrefillArgs& a, cudaStream_t s);
 
+// ---- kv4.cu, kv4_decode.cu, kv4_prefill.cu: the paged cache held in 4 bits (format: kv4.cuh) ---------
+struct Kv4Cache {
+  void* base;       // one layer: uint8 [num_blocks, hkv, record], 16-byte aligned
+  int64_t s_block;  // bytes between blocks (a multiple of 16)
+  int64_t num_blocks;
+  int hkv, d, groups, block_size;
+};
+// RoPE on q/k of qkv [T, (hq + 2 hkv) * d] (+ bias), q to q_out [T, hq, d], k and v quantised into
+// their slots (< 0: not written)
+struct Kv4WriteArgs {
+  Kv4Cache c;
+  const void* qkv;
+  int64_t qkv_stride;  // elements, a multiple of 8
+  const void* bias;    // nullable
+  const int64_t* positions;
+  const float* cos_sin;  // [max_pos, d]
+  int64_t max_pos;
+  const int64_t* slots;
+  void* q_out;
+  int64_t T;
+  int hq;
+  int* status;  // kBadShape: a position or slot out of range (its row was not written)
+};
+cudaError_t launch_rope_kv4(const Kv4WriteArgs& a, cudaStream_t s);
+// the values of the rows at `slots` in bf16: k, v [n, hkv, d] (zeros for a negative slot)
+struct Kv4ReadArgs {
+  Kv4Cache c;
+  const int64_t* slots;
+  void *k, *v;
+  int64_t n;
+  int* status;
+};
+cudaError_t launch_kv4_read(const Kv4ReadArgs& a, cudaStream_t s);
+// decode: one query row per sequence
+struct Kv4DecodeArgs {
+  Kv4Cache c;
+  const void* q;  // [B, hq, d] rows of q_stride elements
+  int64_t q_stride;
+  const int* block_tables;  // [B, bt_cols] rows of bt_stride
+  int64_t bt_stride, bt_cols;
+  const int* ctx_lens;
+  void* out;      // [B, hq, d]
+  float* part_o;  // [B, hq, max_splits, d] (unused with one split)
+  float* part_ml; // [B, hq, max_splits, 2]
+  int* status;
+  int B, hq, max_splits;
+  float scale;
+};
+// splits a history of at most max_len positions is cut into (what part_o and part_ml are sized by)
+int64_t kv4_max_splits(int64_t max_len);
+cudaError_t launch_kv4_decode(const Kv4DecodeArgs& a, cudaStream_t s);
+// pages (blocks) of every layer's cache copied, pairs [n, 2] = (from, to), < 0: padding
+struct CopyPagesArgs {
+  void* const* caches;  // host array of `layers` device addresses
+  int layers;
+  const int64_t* pairs;
+  int64_t n, page_bytes, stride, num_pages;
+  int* status;
+};
+cudaError_t launch_copy_pages(const CopyPagesArgs& a, cudaStream_t s);
+
 // ---- kvcopy.cu -----------------------------------------------------------------------------------
 struct KvCopyArgs {
   const int64_t* layer_ptrs;  // device array of per-layer cache addresses

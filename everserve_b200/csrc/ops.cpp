@@ -675,6 +675,198 @@ void paged_prefill(torch::Tensor q, torch::Tensor cache, torch::Tensor block_tab
   ES_CHECK_CUDA(es::launch_paged_prefill(a, cur()));
 }
 
+// ---- the paged cache held in 4 bits ----------------------------------------------------------------
+
+// A number in a message. (Not streamed: where the toolchain links its C++ library statically beside
+// torch's, streaming a number through the other copy's locale crashes.)
+std::string num(int64_t v) { return std::to_string(v); }
+
+// One layer's cache, uint8 [num_blocks, kv_heads, record]: block size and head dim are the caller's,
+// the groups of a row follow from the record's size (kv4.cuh).
+es::Kv4Cache kv4_cache(const torch::Tensor& cache, int64_t d, int64_t block_size, const torch::Tensor& peer) {
+  TORCH_CHECK(cache.is_cuda() && cache.scalar_type() == at::kByte && cache.dim() == 3,
+              "cache must be uint8 [num_blocks, kv_heads, record] on the device");
+  TORCH_CHECK(cache.device() == peer.device(), "cache and inputs must be on one device");
+  TORCH_CHECK(d == 64 || d == 128, "head_dim must be 64 or 128, got ", num(d));
+  TORCH_CHECK(block_size == 16 || block_size == 32, "block_size must be 16 or 32, got ", num(block_size));
+  const int64_t rec = cache.size(2);
+  const int64_t groups = (rec / block_size - d) / 8;
+  TORCH_CHECK(rec == block_size * (d + 8 * groups) && (groups == 1 || (groups == 2 && d == 128)),
+              "a record of ", num(rec), " bytes is not that of head_dim ", num(d), " and block_size ", num(block_size));
+  TORCH_CHECK(cache.size(1) >= 1 && cache.stride(2) == 1 && (cache.size(1) == 1 || cache.stride(1) == rec),
+              "a block's records must be contiguous");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(cache.data_ptr()) % 16 == 0 &&
+                  (cache.size(0) <= 1 || (cache.stride(0) % 16 == 0 && cache.stride(0) >= cache.size(1) * rec)),
+              "blocks must be 16-byte aligned and apart");
+  es::Kv4Cache c{};
+  c.base = cache.data_ptr();
+  c.s_block = cache.stride(0);
+  c.num_blocks = cache.size(0);
+  c.hkv = (int)cache.size(1);
+  c.d = (int)d;
+  c.groups = (int)groups;
+  c.block_size = (int)block_size;
+  return c;
+}
+
+void on_device_of(const torch::Tensor& t, at::ScalarType st, const torch::Tensor& peer, const char* what) {
+  TORCH_CHECK(t.is_cuda() && t.device() == peer.device() && t.scalar_type() == st, what);
+}
+
+void rope_kv4_write(torch::Tensor qkv, c10::optional<torch::Tensor> bias, torch::Tensor positions,
+                    torch::Tensor cos_sin, torch::Tensor slots, torch::Tensor q_out, torch::Tensor cache, int64_t hq,
+                    int64_t hkv, int64_t block_size, torch::Tensor status) {
+  check_bf16(qkv, "qkv");
+  check_bf16(q_out, "q_out");
+  on_device_of(cos_sin, at::kFloat, qkv, "cos_sin: fp32 [positions, head_dim] on the device of qkv");
+  TORCH_CHECK(cos_sin.dim() == 2 && cos_sin.is_contiguous() && cos_sin.size(0) > 0 &&
+                  reinterpret_cast<uintptr_t>(cos_sin.data_ptr()) % 16 == 0,
+              "cos_sin: contiguous, 16-byte aligned");
+  const int64_t d = cos_sin.size(1);
+  es::Kv4WriteArgs a{};
+  a.c = kv4_cache(cache, d, block_size, qkv);
+  TORCH_CHECK(hq >= 1 && hkv == a.c.hkv, "the cache has ", num(a.c.hkv), " kv heads, not ", num(hkv));
+  TORCH_CHECK(qkv.dim() == 2 && qkv.size(1) == (hq + 2 * hkv) * d, "qkv must be [T, (hq + 2 hkv) * head_dim]");
+  const int64_t T = qkv.size(0);
+  TORCH_CHECK(qkv.stride(1) == 1 && (T <= 1 || (qkv.stride(0) % 8 == 0 && qkv.stride(0) >= qkv.size(1))) &&
+                  reinterpret_cast<uintptr_t>(qkv.data_ptr()) % 16 == 0,
+              "qkv rows must be contiguous and 16-byte aligned");
+  on_device_of(positions, at::kLong, qkv, "positions: int64 on the device of qkv");
+  on_device_of(slots, at::kLong, qkv, "slots: int64 on the device of qkv");
+  TORCH_CHECK(positions.dim() == 1 && positions.is_contiguous() && positions.numel() >= T && slots.dim() == 1 &&
+                  slots.is_contiguous() && slots.numel() >= T,
+              "positions and slots: one contiguous value per row");
+  TORCH_CHECK(q_out.device() == qkv.device() && q_out.is_contiguous() && q_out.numel() == T * hq * d, "q_out must be [T, hq, head_dim]");
+  if (bias.has_value()) {
+    check_bf16(*bias, "bias");
+    TORCH_CHECK(bias->device() == qkv.device() && bias->is_contiguous() && bias->numel() == qkv.size(1) &&
+                    reinterpret_cast<uintptr_t>(bias->data_ptr()) % 16 == 0,
+                "bias must be a contiguous, 16-byte aligned row");
+    a.bias = bias->data_ptr();
+  }
+  on_device_of(status, at::kInt, qkv, "status must be int32 on the device of qkv");
+  a.qkv = qkv.data_ptr();
+  a.qkv_stride = qkv.stride(0);
+  a.positions = positions.data_ptr<int64_t>();
+  a.cos_sin = cos_sin.data_ptr<float>();
+  a.max_pos = cos_sin.size(0);
+  a.slots = slots.data_ptr<int64_t>();
+  a.q_out = q_out.data_ptr();
+  a.T = T;
+  a.hq = (int)hq;
+  a.status = status.data_ptr<int>();
+  const c10::cuda::CUDAGuard g(qkv.device());
+  ES_CHECK_CUDA(es::launch_rope_kv4(a, cur()));
+}
+
+void kv4_read(torch::Tensor cache, torch::Tensor slots, torch::Tensor k, torch::Tensor v, int64_t d,
+              int64_t block_size, torch::Tensor status) {
+  check_bf16(k, "k");
+  check_bf16(v, "v");
+  es::Kv4ReadArgs a{};
+  a.c = kv4_cache(cache, d, block_size, k);
+  on_device_of(slots, at::kLong, cache, "slots: int64 on the device of the cache");
+  TORCH_CHECK(slots.dim() == 1 && slots.is_contiguous(), "slots: one contiguous value per row");
+  const int64_t n = slots.numel();
+  TORCH_CHECK(k.is_contiguous() && v.is_contiguous() && v.device() == k.device() && k.numel() == n * a.c.hkv * d &&
+                  v.numel() == k.numel(),
+              "k and v must be [n, kv_heads, head_dim]");
+  on_device_of(status, at::kInt, cache, "status must be int32 on the device of the cache");
+  a.slots = slots.data_ptr<int64_t>();
+  a.k = k.data_ptr();
+  a.v = v.data_ptr();
+  a.n = n;
+  a.status = status.data_ptr<int>();
+  const c10::cuda::CUDAGuard g(cache.device());
+  ES_CHECK_CUDA(es::launch_kv4_read(a, cur()));
+}
+
+void paged_decode_kv4(torch::Tensor q, torch::Tensor cache, torch::Tensor block_tables, torch::Tensor ctx_lens,
+                      torch::Tensor out, torch::Tensor part_o, torch::Tensor part_ml, torch::Tensor status,
+                      int64_t block_size, int64_t max_splits, double scale) {
+  check_bf16(q, "q");
+  check_bf16(out, "out");
+  TORCH_CHECK(q.dim() == 3, "q must be [B, hq, head_dim]");
+  const int64_t B = q.size(0), hq = q.size(1), d = q.size(2);
+  es::Kv4DecodeArgs a{};
+  a.c = kv4_cache(cache, d, block_size, q);
+  TORCH_CHECK(hq >= 1 && hq % a.c.hkv == 0, "query heads must be a multiple of the cache's kv heads");
+  TORCH_CHECK(q.stride(2) == 1 && (hq == 1 || q.stride(1) == d) &&
+                  (B <= 1 || (q.stride(0) % 8 == 0 && q.stride(0) >= hq * d)) &&
+                  reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0,
+              "q rows must be contiguous and 16-byte aligned");
+  TORCH_CHECK(out.device() == q.device() && out.is_contiguous() && out.sizes() == q.sizes() &&
+                  reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0,
+              "out must be [B, hq, head_dim]");
+  on_device_of(block_tables, at::kInt, q, "block_tables: int32 on the device of q");
+  on_device_of(ctx_lens, at::kInt, q, "ctx_lens: int32 on the device of q");
+  TORCH_CHECK(block_tables.dim() == 2 && block_tables.stride(1) == 1 && block_tables.size(0) >= B &&
+                  ctx_lens.dim() == 1 && ctx_lens.is_contiguous() && ctx_lens.numel() >= B,
+              "block_tables [B, blocks] and ctx_lens [B], rows contiguous");
+  TORCH_CHECK(B == 0 || (a.c.num_blocks > 0 && block_tables.size(1) > 0), "an empty cache or block table");
+  on_device_of(part_o, at::kFloat, q, "part_o: fp32 on the device of q");
+  on_device_of(part_ml, at::kFloat, q, "part_ml: fp32 on the device of q");
+  TORCH_CHECK(max_splits >= 1 && max_splits <= INT32_MAX &&
+                  (max_splits == 1 || (part_o.is_contiguous() && part_ml.is_contiguous() &&
+                                       part_o.numel() >= B * hq * max_splits * d &&
+                                       part_ml.numel() >= B * hq * max_splits * 2)),
+              "split scratch too small");
+  on_device_of(status, at::kInt, q, "status must be int32 on the device of q");
+  a.q = q.data_ptr();
+  a.q_stride = q.stride(0);
+  a.block_tables = block_tables.data_ptr<int>();
+  a.bt_stride = block_tables.stride(0);
+  a.bt_cols = block_tables.size(1);
+  a.ctx_lens = ctx_lens.data_ptr<int>();
+  a.out = out.data_ptr();
+  a.part_o = part_o.data_ptr<float>();
+  a.part_ml = part_ml.data_ptr<float>();
+  a.status = status.data_ptr<int>();
+  a.B = (int)B;
+  a.hq = (int)hq;
+  a.max_splits = (int)max_splits;
+  a.scale = (float)scale;
+  const c10::cuda::CUDAGuard g(q.device());
+  ES_CHECK_CUDA(es::launch_kv4_decode(a, cur()));
+}
+
+// caches[l][pairs[i, 1]] = caches[l][pairs[i, 0]]: pages are the first dimension, contiguous inside
+void copy_pages(std::vector<torch::Tensor> caches, torch::Tensor pairs, torch::Tensor status) {
+  if (caches.empty()) return;
+  const torch::Tensor& c0 = caches[0];
+  TORCH_CHECK(c0.is_cuda() && c0.dim() >= 2, "caches: tensors with pages along the first dimension, on the device");
+  std::vector<void*> ptrs;
+  ptrs.reserve(caches.size());
+  for (const torch::Tensor& c : caches) {
+    TORCH_CHECK(c.device() == c0.device() && c.scalar_type() == c0.scalar_type() && c.sizes() == c0.sizes() &&
+                    c.strides() == c0.strides(),
+                "the layers' caches must be alike");
+    ptrs.push_back(c.data_ptr());
+  }
+  int64_t inner = 1;
+  for (int64_t i = c0.dim() - 1; i >= 1; i--) {
+    TORCH_CHECK(c0.size(i) == 1 || c0.stride(i) == inner, "a page must be contiguous");
+    inner *= c0.size(i);
+  }
+  TORCH_CHECK(c0.size(0) <= 1 || c0.stride(0) >= inner, "pages must not overlap");
+  on_device_of(pairs, at::kLong, c0, "pairs: int64 [n, 2] on the device of the caches");
+  TORCH_CHECK(pairs.dim() == 2 && pairs.size(1) == 2 && pairs.is_contiguous(), "pairs: contiguous [n, 2] of (from, to)");
+  on_device_of(status, at::kInt, c0, "status must be int32 on the device of the caches");
+  const int64_t elem = c0.element_size();
+  TORCH_CHECK(inner * elem % 16 == 0 && c0.stride(0) * elem % 16 == 0, "a page must be a multiple of 16 bytes");
+  es::CopyPagesArgs a{};
+  a.caches = ptrs.data();
+  a.layers = (int)ptrs.size();
+  a.pairs = pairs.data_ptr<int64_t>();
+  a.n = pairs.size(0);
+  a.page_bytes = inner * elem;
+  a.stride = c0.stride(0) * elem;
+  a.num_pages = c0.size(0);
+  a.status = status.data_ptr<int>();
+  const c10::cuda::CUDAGuard g(c0.device());
+  ES_CHECK_CUDA(es::launch_copy_pages(a, cur()));
+}
+
 void kv_copy(bool gather, torch::Tensor layer_ptrs, torch::Tensor slots, torch::Tensor heads, int64_t staging_ptr,
              int64_t cap, int64_t d, int64_t block_size, std::vector<int64_t> strides, int64_t elem) {
   TORCH_CHECK(layer_ptrs.is_cuda() && slots.is_cuda() && heads.is_cuda(), "device index tensors");
@@ -873,6 +1065,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("quant_fp8", &quant_fp8, "x -> e4m3 with a scale per token and 128-wide block");
   m.def("gemm_fp8", &gemm_fp8, "block-scaled fp8 GEMM (tcgen05 kind::f8f6f4, scales per 128-wide K block)");
   m.def("paged_prefill", &paged_prefill, "paged causal prefill attention (tcgen05: S and P.V in TMEM, TMA K/V tiles)");
+  m.def("rope_kv4_write", &rope_kv4_write, "RoPE on q/k and the write of k/v into the paged cache held in 4 bits");
+  m.def("kv4_read", &kv4_read, "values of rows of the paged cache held in 4 bits");
+  m.def("paged_decode_kv4", &paged_decode_kv4, "decode attention over the paged cache held in 4 bits");
+  m.def("kv4_max_splits", &es::kv4_max_splits, "splits of a history of at most max_len positions");
+  m.def("copy_pages", &copy_pages, "pages copied in every layer's cache, one launch");
   m.def("moe_route", &moe_route, "mixture routing: per-token weights of this rank's experts [el, T]");
   m.def("moe_topk", &moe_topk, "mixture routing: each token's top k experts and their weights");
   m.def("moe_dispatch", &moe_dispatch, "expert-parallel dispatch of tokens to their experts' owners (peer stores)");

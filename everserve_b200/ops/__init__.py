@@ -64,6 +64,23 @@ class RefOps:
     def prefill_attention(self, q, cache, block_tables, ctx_lens, q_seq, q_pos, scale, tiles=None):
         return ref.paged_attention(q, cache, block_tables, ctx_lens, q_seq, q_pos, scale)
 
+    def rope_kv4_write(self, qkv, bias, positions, cos_sin, slots, cache, hq, hkv, block_size):
+        return ref.rope_kv4_write(qkv, bias, positions, cos_sin, slots, cache, hq, hkv, block_size)
+
+    def kv4_read(self, cache, slots, head_dim, block_size):
+        return ref.kv4_read(cache, slots, head_dim, block_size)
+
+    def decode_attention_kv4(self, q, cache, block_tables, ctx_lens, scale, block_size, max_model_len=None):
+        rows = torch.arange(q.shape[0], device=q.device)
+        return ref.kv4_attention(q, cache, block_tables, ctx_lens[: q.shape[0]], rows, scale, block_size)
+
+    def prefill_attention_kv4(self, q, cache, block_tables, ctx_lens, last_rows, scale, block_size):
+        return ref.kv4_attention(q, cache, block_tables, ctx_lens, last_rows, scale, block_size)
+
+    def copy_pages(self, caches, pairs):
+        check_pairs(pairs)
+        ref.copy_pages(caches, pairs)
+
     def silu_mul(self, gu, interleaved: bool = False):
         if interleaved:
             gu = deinterleave_gate_up(gu.t()).t()
@@ -250,6 +267,42 @@ class KernelOps:
         self.C.paged_prefill(qc, cache, block_tables, tiles, out, self.status, scale)
         return out
 
+    # ---- the paged cache held in 4 bits (format: ref.kv4_cache_shape and above) -------------------
+    def rope_kv4_write(self, qkv, bias, positions, cos_sin, slots, cache, hq, hkv, block_size):
+        """RoPE on q and k, k and v quantised to 4 bits into their slots of `cache` (uint8, of
+        ``ref.kv4_cache_shape``); returns q [T, hq, d]. A negative slot is not written; a position or
+        slot out of range is reported by ``check_status``."""
+        q = torch.empty(qkv.shape[0], hq, cos_sin.shape[1], dtype=qkv.dtype, device=qkv.device)
+        self.C.rope_kv4_write(qkv, bias, positions, cos_sin, slots, q, cache, hq, hkv, block_size, self.status)
+        return q
+
+    def kv4_read(self, cache, slots, head_dim, block_size):
+        """The rows at `slots` (int64 [n]) as bf16 k, v [n, kv_heads, head_dim]; zeros for a negative slot."""
+        kv = torch.empty(2, slots.shape[0], cache.shape[1], head_dim, dtype=torch.bfloat16, device=cache.device)
+        self.C.kv4_read(cache, slots, kv[0], kv[1], head_dim, block_size, self.status)
+        return kv[0], kv[1]
+
+    def decode_attention_kv4(self, q, cache, block_tables, ctx_lens, scale, block_size, max_model_len=None):
+        """Attention of one query row per sequence over its history in 4 bits: q [B, hq, d] -> [B, hq, d];
+        an empty history gives zeros. The result of a sequence does not depend on its batch. The
+        workspace is the call's own, so calls on several streams do not meet in it."""
+        B, hq, d = q.shape
+        if max_model_len is None:
+            max_model_len = block_tables.shape[1] * block_size
+        ms = int(self.C.kv4_max_splits(max_model_len))
+        out = torch.empty(B, hq, d, dtype=q.dtype, device=q.device)
+        part = torch.empty(B * hq * ms * (d + 2) if ms > 1 else 0, dtype=torch.float32, device=q.device)
+        n = B * hq * ms * d if ms > 1 else 0
+        self.C.paged_decode_kv4(q, cache, block_tables, ctx_lens, out, part[:n], part[n:], self.status, block_size, ms,
+                                scale)
+        return out
+
+    def copy_pages(self, caches, pairs):
+        """Copy pages (the first dimension's entries) in every layer's cache, bf16 or 4-bit: pairs int64
+        [n, 2] of (from, to) on the device, negative entries padding. One launch; the pairs are copied in
+        no order, so no page may be both copied from and to, nor be copied to twice."""
+        self.C.copy_pages(caches, pairs, self.status)
+
     def silu_mul(self, gu, interleaved: bool = False):
         out = torch.empty(*gu.shape[:-1], gu.shape[-1] // 2, dtype=gu.dtype, device=gu.device)
         self.C.silu_mul(gu, out, interleaved)
@@ -291,6 +344,15 @@ class KernelOps:
         if v:
             self.status.zero_()
         return v
+
+
+def check_pairs(pairs: torch.Tensor) -> None:
+    """A page copy's (from, to) pairs on the host: raise where the pages' final content would depend on
+    the order of the copies."""
+    rows = [(int(a), int(b)) for a, b in pairs.tolist() if a >= 0 and b >= 0]
+    to = {b for _, b in rows}
+    if len(to) != len(rows) or to & {a for a, _ in rows}:
+        raise ValueError("a page is copied to twice, or both copied from and to")
 
 
 FP8_MAX = 448.0  # largest finite e4m3

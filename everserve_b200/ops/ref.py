@@ -128,6 +128,132 @@ def paged_attention(q, cache, block_tables, ctx_lens, q_seq, q_pos, scale: float
     return out
 
 
+# ---- the paged cache held in 4 bits (one layer: uint8 [num_blocks, kv_heads, record]) ---------------
+#
+# A group is 64 channels, or the whole head, of one row (one token's K or V of one kv head). With mn and
+# mx its smallest and largest value: scale = bf16((mx - mn) / 15), zero = bf16(mn), code =
+# clamp(round((x - zero) / scale), 0, 15), and the value held is scale * code + zero (a group of equal
+# values has scale 0). A group holding a value that is not finite reads as NaN. A record holds the K
+# codes [bs, d / 2], the V codes, the K pairs (scale, zero) [bs, groups, 2] in bf16, the V pairs.
+
+
+def kv4_cache_shape(num_blocks: int, kv_heads: int, block_size: int, head_dim: int, group: int = 64) -> tuple[int, int, int]:
+    """Shape of one layer's cache in 4 bits (uint8); `group`: channels that share a scale, 64 or head_dim."""
+    if head_dim not in (64, 128) or group not in (64, head_dim) or block_size not in (16, 32):
+        raise ValueError(f"no 4-bit cache of head_dim {head_dim}, group {group}, block_size {block_size}")
+    return num_blocks, kv_heads, block_size * (head_dim + 8 * (head_dim // group))
+
+
+def kv4_groups(cache: torch.Tensor, head_dim: int, block_size: int) -> int:
+    """Groups of a row, from the size of the cache's records."""
+    groups = (cache.shape[2] // block_size - head_dim) // 8
+    if groups < 1 or kv4_cache_shape(cache.shape[0], cache.shape[1], block_size, head_dim, head_dim // groups) != tuple(cache.shape):
+        raise ValueError(f"a record of {cache.shape[2]} bytes is not that of head_dim {head_dim}, block_size {block_size}")
+    return groups
+
+
+def kv4_order(head_dim: int, device=None) -> torch.Tensor:
+    """The channel of each stored nibble of a row (byte by byte, the low nibble first)."""
+    p = torch.arange(head_dim // 8, device=device)
+    word = p // 2 + 8 * (p % 2) if head_dim == 128 else p
+    return (8 * word[:, None] + torch.tensor([0, 2, 4, 6, 1, 3, 5, 7], device=device)).reshape(-1)
+
+
+def kv4_quantize(x: torch.Tensor, groups: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """x [..., d] -> (stored codes uint8 [..., d / 2], (scale, zero) bf16 [..., groups, 2])."""
+    d = x.shape[-1]
+    g = x.float().unflatten(-1, (groups, d // groups))
+    mn, mx = g.amin(-1, keepdim=True), g.amax(-1, keepdim=True)
+    scale, zero = ((mx - mn) * (1.0 / 15.0)).bfloat16(), mn.bfloat16()
+    s = scale.float()
+    code = torch.round((g - zero.float()) / torch.where(s > 0, s, torch.ones_like(s))).nan_to_num().clamp(0, 15)
+    code = torch.where(s > 0, code, torch.zeros_like(code)).flatten(-2).to(torch.uint8)
+    pair = code[..., kv4_order(d, x.device)].unflatten(-1, (d // 2, 2))
+    scale = torch.where(torch.isfinite(g).all(-1, keepdim=True), scale, torch.full_like(scale, math.nan))
+    return pair[..., 0] | (pair[..., 1] << 4), torch.cat([scale, zero], -1)
+
+
+def kv4_parts(cache: torch.Tensor, head_dim: int, block_size: int) -> list[torch.Tensor]:
+    """Views of the cache's bytes: K codes, V codes [nb, hkv, bs, d / 2], K pairs, V pairs [nb, hkv, bs, 4 * groups]."""
+    n, m = block_size * head_dim // 2, 4 * block_size * kv4_groups(cache, head_dim, block_size)
+    return [t.unflatten(-1, (block_size, -1)) for t in cache.split((n, n, m, m), -1)]
+
+
+def kv4_values(codes: torch.Tensor, pairs: torch.Tensor) -> torch.Tensor:
+    """The fp32 values of stored rows: codes [..., d / 2], pairs [..., 4 * groups] (bytes) -> [..., d]."""
+    d = 2 * codes.shape[-1]
+    nib = torch.stack((codes & 15, codes >> 4), -1).flatten(-2).float()
+    x = torch.empty_like(nib)
+    x[..., kv4_order(d, codes.device)] = nib
+    sz = pairs.contiguous().view(torch.bfloat16).unflatten(-1, (-1, 2)).float()
+    groups = sz.shape[-2]
+    return (x.unflatten(-1, (groups, d // groups)) * sz[..., :1] + sz[..., 1:]).flatten(-2)
+
+
+def kv4_read(cache: torch.Tensor, slots: torch.Tensor, head_dim: int, block_size: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """The fp32 rows at `slots` of a cache in 4 bits: k, v [n, hkv, d]; zeros for a negative slot."""
+    kc, vc, kp, vp = kv4_parts(cache, head_dim, block_size)
+    s = slots.clamp(min=0)
+    blk, off = s // block_size, s % block_size
+    keep = (slots >= 0)[:, None, None]
+    zero = torch.zeros((), device=cache.device)
+    return tuple(torch.where(keep, kv4_values(c[blk, :, off], p[blk, :, off]), zero) for c, p in ((kc, kp), (vc, vp)))
+
+
+def kv4_cache_values(cache: torch.Tensor, head_dim: int, block_size: int) -> torch.Tensor:
+    """Every value a cache in 4 bits holds, as an fp32 cache [num_blocks, 2, hkv, bs, d]."""
+    kc, vc, kp, vp = kv4_parts(cache, head_dim, block_size)
+    return torch.stack((kv4_values(kc, kp), kv4_values(vc, vp)), 1)
+
+
+def rope_kv4_write(qkv, bias, positions, cos_sin, slots, cache, hq: int, hkv: int, block_size: int) -> torch.Tensor:
+    """Rotate q and k, quantise k and v into the slots of a cache in 4 bits; return q as [T, hq, d]."""
+    T, d = qkv.shape[0], cos_sin.shape[1]
+    x = qkv.float()
+    if bias is not None:
+        x = x + bias.float()
+    x = x.view(T, hq + 2 * hkv, d)
+    qk = rope(x[:, : hq + hkv], cos_sin[positions])
+    keep = slots >= 0
+    blk, off = slots[keep] // block_size, slots[keep] % block_size
+    kc, vc, kp, vp = kv4_parts(cache, d, block_size)
+    groups = kv4_groups(cache, d, block_size)
+    for rows, codes, pairs in ((qk[:, hq:], kc, kp), (x[:, hq + hkv :], vc, vp)):
+        c, p = kv4_quantize(rows[keep], groups)
+        codes[blk, :, off] = c
+        pairs[blk, :, off] = p.flatten(-2).contiguous().view(torch.uint8)
+    return qk[:, :hq].to(qkv.dtype)
+
+
+def kv4_attention(q, cache, block_tables, ctx_lens, last_rows, scale: float, block_size: int) -> torch.Tensor:
+    """Causal attention over a cache in 4 bits. q [T, hq, d]: sequence s owns the rows up to last_rows[s],
+    and its last one sits at position ctx_lens[s] - 1; a row without a visible key is zero."""
+    T, hq, d = q.shape
+    out = torch.zeros_like(q)
+    kc, vc, kp, vp = kv4_parts(cache, d, block_size)
+    r0 = 0
+    for s, (last, n) in enumerate(zip(last_rows.tolist(), ctx_lens.tolist())):
+        r1 = last + 1
+        if n > 0 and r1 > r0:
+            blk = block_tables[s, : (n + block_size - 1) // block_size].long()
+            k, v = (kv4_values(c[blk], p[blk]).transpose(1, 2).flatten(0, 1)[:n].repeat_interleave(hq // cache.shape[1], 1)
+                    for c, p in ((kc, kp), (vc, vp)))
+            score = torch.einsum("thd,nhd->htn", q[r0:r1].float(), k) * scale
+            pos = torch.arange(n - (r1 - r0), n, device=q.device)
+            score = score.masked_fill((torch.arange(n, device=q.device)[None] > pos[:, None])[None], float("-inf"))
+            o = torch.einsum("htn,nhd->thd", torch.softmax(score, -1), v)
+            out[r0:r1] = torch.where((pos >= 0)[:, None, None], o, torch.zeros_like(o)).to(q.dtype)
+        r0 = r1
+    return out
+
+
+def copy_pages(caches: list[torch.Tensor], pairs: torch.Tensor) -> None:
+    """caches[l][to] = caches[l][from] for every layer and (from, to) of pairs [n, 2]; negative: padding."""
+    p = pairs[(pairs >= 0).all(1)]
+    for c in caches:
+        c[p[:, 1]] = c[p[:, 0]]
+
+
 def silu_mul(gu: torch.Tensor) -> torch.Tensor:
     inter = gu.shape[-1] // 2
     g, u = gu[..., :inter].float(), gu[..., inter:].float()
