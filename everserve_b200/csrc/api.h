@@ -287,6 +287,28 @@ struct Kv4DecodeArgs {
 // splits a history of at most max_len positions is cut into (what part_o and part_ml are sized by)
 int64_t kv4_max_splits(int64_t max_len);
 cudaError_t launch_kv4_decode(const Kv4DecodeArgs& a, cudaStream_t s);
+// prefill: causal attention of T new rows of S sequences; sequence s owns the rows up to last_rows[s], the
+// last of them at position ctx_lens[s] - 1
+struct Kv4PrefillArgs {
+  Kv4Cache c;
+  const void* q;  // [T, hq, d] rows of q_stride elements
+  int64_t q_stride;
+  const int* block_tables;  // [S, bt_cols] rows of bt_stride
+  int64_t bt_stride, bt_cols;
+  const int* ctx_lens;
+  const int64_t* last_rows;
+  void* out;       // [T, hq, d]
+  float* part_o;   // [T, hq, max_splits, d] (unused with one split)
+  float* part_ml;  // [T, hq, max_splits, 2]
+  int* part_ns;    // [T]
+  int* status;
+  int64_t T, S;
+  int hq, max_splits, num_sms;
+  float scale;
+};
+// splits a row of such a step may be cut into, with no context above max_len
+int64_t kv4_prefill_splits(int64_t T, int64_t S, int64_t hq, int64_t hkv, int64_t max_len);
+cudaError_t launch_kv4_prefill(const Kv4PrefillArgs& a, cudaStream_t s);
 // pages (blocks) of every layer's cache copied, pairs [n, 2] = (from, to), < 0: padding
 struct CopyPagesArgs {
   void* const* caches;  // host array of `layers` device addresses

@@ -39,6 +39,13 @@ struct Rec {
 ES_DEVICE float pair_scale(uint32_t p) { return __uint_as_float(p << 16); }
 ES_DEVICE float pair_zero(uint32_t p) { return __uint_as_float(p & 0xFFFF0000u); }
 
+// 2^x by the hardware's approximation (2^-22 relative); 0 below 2^-126
+ES_DEVICE float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // Calls f with a cache's (head dim, groups, block size) as integral constants; refuses others.
 template <typename F>
 cudaError_t pick(int d, int groups, int bs, F&& f) {

@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(kDecThreads) decode_kernel(DecodeParams p) {
 #pragma unroll
       for (int j = 0; j < 2; j++) {
         const float mn = fmaxf(m[j], mt[j]);
-        c[j] = m[j] == -INFINITY ? 0.f : exp2f(m[j] - mn);
+        c[j] = m[j] == -INFINITY ? 0.f : ex2(m[j] - mn);
         m[j] = mn;
         l[j] *= c[j];
 #pragma unroll
@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(kDecThreads) decode_kernel(DecodeParams p) {
     for (int i = 0; i < 2; i++)
 #pragma unroll
       for (int j = 0; j < 2; j++) {
-        pr[i][j] = exp2f(x[i][j] - m[j]);
+        pr[i][j] = ex2(x[i][j] - m[j]);
         l[j] += pr[i][j];
 #pragma unroll
         for (int g = 0; g < NG; g++) zs[j][g] = fmaf(pr[i][j], zv[i][g], zs[j][g]);
@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(kDecThreads) decode_kernel(DecodeParams p) {
     for (int w = 0; w < kDecWarps; w++) {
       if (s0 + w * 16 >= s1) continue;  // a warp with no key
       const float mw = red_ml[w][h][0];
-      const float f = mw == mm ? 1.f : exp2f(mw - mm);
+      const float f = mw == mm ? 1.f : ex2(mw - mm);
       ll = fmaf(red_ml[w][h][1], f, ll);
 #pragma unroll
       for (int e = 0; e < 8; e++) acc[e] = fmaf(red_o[w][h][c8 + e], f, acc[e]);
@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(128) merge_kernel(const float* __restrict__ pa
   for (int e = 0; e < E; e++) acc[e] = 0.f;
   for (int i = warp; i < ns; i += 4) {
     const float mi = ml[2 * i];
-    const float f = mi == mx ? 1.f : exp2f(mi - mx);
+    const float f = mi == mx ? 1.f : ex2(mi - mx);
     l = fmaf(ml[2 * i + 1], f, l);
     const float* po = part_o + (row * max_splits + i) * D;
 #pragma unroll

@@ -1,0 +1,553 @@
+// Causal attention of a step's new rows over their sequences' paged history held in 4 bits (tcgen05, TMEM).
+//
+// The products are large here (128 and more query rows share a key), so a key's codes are turned into
+// bf16 values once for 256 query rows and the tensor cores do the rest: v = scale * c + zero, c exact in
+// bf16 and the multiply-add rounded once. The query rows of one kv head's whole group are packed into the
+// rows of a tile (row = token * G + head of the group), so grouped heads share the conversion too.
+//
+// A CTA keeps to its SM and walks work items: 256 rows (two tiles of 128) of one sequence and kv head,
+// over a run of 128-key tiles. Its warps:
+//   * 8-11 turn tile j's codes (loaded a tile ahead, straight to registers) into K and V stages in shared
+//     memory, 128-byte swizzled;
+//   * 12 issues the MMAs: S_t = Q_t . K_j^T and O_t += P_t . V_j for t = 0, 1 in turn, P read from TMEM;
+//   * 0-3 and 4-7 do the softmax of tiles 0 and 1, a thread a row: S from TMEM, P back over it in bf16.
+// While one tile's softmax runs, the tensor core works for the other. The running maximum moves (and O in
+// TMEM is rescaled) only when a score passes it by 2^8, so most tiles leave O alone. A row's sums are fp32.
+//
+// A sequence with few rows and a long history is cut along its keys as well, into items whose results
+// (O, m, l) a second kernel joins. The cut depends on the sequence's own rows and keys and on the model's
+// heads, never on the batch. Each warp finds its item by a scan over the sequences, so the host needs no
+// plan and no synchronisation. All waits are bounded and end in the status word.
+#include <atomic>
+
+#include "api.h"
+#include "common.cuh"
+#include "kv4.cuh"
+#include "launch.h"
+#include "ptx.cuh"
+
+namespace es {
+namespace kv4 {
+
+constexpr int kRows = 128;  // rows of a tile (MMA M)
+constexpr int kKeys = 128;  // keys of a tile (MMA N of S, K of P.V)
+constexpr int kSoftThreads = 256;
+constexpr int kConvThreads = 128;
+constexpr int kPreThreads = kSoftThreads + kConvThreads + 32;
+constexpr int kTmem = 512;  // S0, S1 (128 columns each, P over them), O0, O1
+
+template <int D>
+struct PreCfg {
+  static constexpr int kChunk = kRows * 128;           // one 64-channel chunk of a 128-row operand
+  static constexpr int kTile = (D / 64) * kChunk;      // a bf16 tile of 128 rows
+  static constexpr int kSmem = 1024 + 2 * kTile + 2 * 2 * kTile + 256;
+};
+
+struct PreParams {
+  const __nv_bfloat16* q;  // [T, hq, D] rows of q_stride
+  int64_t q_stride;
+  const uint8_t* cache;
+  int64_t s_block, num_blocks;
+  const int* block_tables;
+  int64_t bt_stride;
+  int bt_cols;
+  const int* ctx_lens;
+  const int64_t* last_rows;
+  __nv_bfloat16* out;  // [T, hq, D]
+  float* part_o;       // [T, hq, max_splits, D]
+  float* part_ml;      // [T, hq, max_splits, 2]
+  int* part_ns;        // [T]
+  int* status;
+  int T, S, hq, hkv, G, tt, max_splits;  // tt: tokens of a 128-row tile
+  float scale_log2;
+};
+
+// Key tiles of one item for a sequence of `tiles` row tiles: all of them where its items fill the SMs
+// without a cut.
+__host__ __device__ __forceinline__ int chunk_of(int tiles, int hkv) {
+  const int items = tiles * hkv;
+  return items >= 128 ? 1 << 24 : items > 16 ? 16 : 8;
+}
+
+struct Item {
+  int seq, rows, row0, ctx;  // the sequence, its rows, its first row, its context length
+  int tile, head, split, chunk;
+};
+
+// Work item `idx`, in an order that starts with a sequence's last (longest) tiles; false: there is none.
+// The whole warp calls it.
+ES_DEVICE bool find_item(const PreParams& p, int bs, int idx, Item& it) {
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  for (int s0 = 0; s0 < p.S; s0 += 32) {
+    const int s = s0 + lane;
+    int rows = 0, r0 = 0, ctx = 0, tiles = 0, ns = 0, chunk = 1, items = 0;
+    if (s < p.S) {
+      const int64_t T = p.T;
+      r0 = s == 0 ? 0 : (int)max((int64_t)0, min(T, p.last_rows[s - 1] + 1));
+      rows = max(0, (int)min(T, p.last_rows[s] + 1) - r0);
+      ctx = min(p.ctx_lens[s], p.bt_cols * bs);
+      tiles = (rows + 2 * p.tt - 1) / (2 * p.tt);
+      chunk = chunk_of(tiles, p.hkv);
+      ns = max(1, min(p.max_splits, ((ctx + kKeys - 1) / kKeys + chunk - 1) / chunk));
+      items = tiles * ns * p.hkv;
+    }
+    int upto = items;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    const int total = __shfl_sync(0xffffffffu, upto, 31);
+    if (idx < before + total) {
+      const int src = __ffs(__ballot_sync(0xffffffffu, idx < before + upto)) - 1;
+      const int first = before + __shfl_sync(0xffffffffu, upto - items, src);
+      it.seq = s0 + src;
+      it.rows = __shfl_sync(0xffffffffu, rows, src);
+      it.row0 = __shfl_sync(0xffffffffu, r0, src);
+      it.ctx = __shfl_sync(0xffffffffu, ctx, src);
+      it.chunk = __shfl_sync(0xffffffffu, chunk, src);
+      const int t = __shfl_sync(0xffffffffu, tiles, src), per = __shfl_sync(0xffffffffu, ns, src) * p.hkv;
+      const int at = idx - first;
+      it.tile = t - 1 - at / per;
+      it.split = at % per / p.hkv;
+      it.head = at % per % p.hkv;
+      return true;
+    }
+    before += total;
+  }
+  return false;
+}
+
+// The key tiles [j0, j1) of an item, and how many items its row tile has.
+ES_DEVICE void span(const PreParams& p, const Item& it, int& j0, int& j1, int& ns) {
+  const int last = min(it.rows, (it.tile + 1) * 2 * p.tt) - 1;  // the tile's last token
+  const int pos = min(it.ctx - it.rows + last, it.ctx - 1);
+  const int J = pos < 0 ? 0 : pos / kKeys + 1;
+  ns = max(1, min(p.max_splits, (J - 1) / it.chunk + 1));
+  j0 = it.split * it.chunk;
+  j1 = it.split == ns - 1 ? J : min(J, j0 + it.chunk);
+  if (it.split >= ns) j1 = j0;
+}
+
+// 8 codes -> 8 bf16 values
+ES_DEVICE uint4 values8(uint32_t w, __nv_bfloat162 s, __nv_bfloat162 z) {
+  const __nv_bfloat162 bias = __floats2bfloat162_rn(128.f, 128.f);
+  uint32_t r[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const uint32_t h = ((w >> (4 * j)) & 0x000F000Fu) | 0x43004300u;  // 128 + c
+    const __nv_bfloat162 c = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&h), bias);
+    const __nv_bfloat162 v = __hfma2(c, s, z);
+    r[j] = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+// What a converting thread holds of a key tile: 16-byte pieces (32 codes) of K and of V rows.
+template <int D, int NG>
+struct Raw {
+  static constexpr int kPer = D / 32;  // pieces of a row, and passes over the 128 rows
+  uint4 k[kPer], v[kPer];
+  uint32_t km[kPer][NG], vm[kPer][NG];
+};
+
+template <int D, int NG, int BS>
+ES_DEVICE void load_raw(Raw<D, NG>& r, const PreParams& p, const Item& it, int j, int tid) {
+  using R = Rec<D, NG, BS>;
+  constexpr int P = D / 32;
+  const int* bt = p.block_tables + (int64_t)it.seq * p.bt_stride;
+#pragma unroll
+  for (int i = 0; i < P; i++) {
+    const int key = j * kKeys + i * (kConvThreads / P) + tid / P;
+    r.k[i] = r.v[i] = make_uint4(0, 0, 0, 0);  // past the history: values of zero, whatever the slot holds
+#pragma unroll
+    for (int g = 0; g < NG; g++) r.km[i][g] = r.vm[i][g] = 0;
+    if (key < it.ctx) {
+      int64_t blk = bt[key / BS];
+      if (blk < 0 || blk >= p.num_blocks) {  // not a block of this cache: reported, block 0 read instead
+        if (p.status) atomicExch(p.status, (int)kBadShape);
+        blk = 0;
+      }
+      const uint8_t* rec = p.cache + blk * p.s_block + (int64_t)it.head * R::kBytes;
+      const int off = key % BS;
+      r.k[i] = *reinterpret_cast<const uint4*>(rec + off * R::kRow + 16 * (tid % P));
+      r.v[i] = *reinterpret_cast<const uint4*>(rec + R::kV + off * R::kRow + 16 * (tid % P));
+      const uint32_t* km = reinterpret_cast<const uint32_t*>(rec + R::kKMeta + off * R::kMeta);
+      const uint32_t* vm = reinterpret_cast<const uint32_t*>(rec + R::kVMeta + off * R::kMeta);
+#pragma unroll
+      for (int g = 0; g < NG; g++) r.km[i][g] = km[g], r.vm[i][g] = vm[g];
+    }
+  }
+}
+
+// One piece of row `row` into a tile's swizzled layout.
+template <int D, int NG>
+ES_DEVICE void store_piece(uint8_t* tile, int row, int piece, const uint4& codes, const uint32_t* meta) {
+  const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+  __nv_bfloat162 s[NG], z[NG];
+#pragma unroll
+  for (int g = 0; g < NG; g++) {
+    const uint32_t sp = __byte_perm(meta[g], meta[g], 0x1010), zp = __byte_perm(meta[g], meta[g], 0x3232);
+    s[g] = *reinterpret_cast<const __nv_bfloat162*>(&sp);
+    z[g] = *reinterpret_cast<const __nv_bfloat162*>(&zp);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int chunk = D == 128 ? (i & 1) : 0;
+    const int unit = D == 128 ? 2 * piece + (i >> 1) : 4 * piece + i;
+    const int g = NG == 2 ? chunk : 0;
+    *reinterpret_cast<uint4*>(tile + chunk * PreCfg<D>::kChunk + row * 128 + ((unit ^ (row & 7)) << 4)) =
+        values8(w[i], s[g], z[g]);
+  }
+}
+
+template <int D, int NG, int BS>
+__global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
+  using C = PreCfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* q_s = smem;                  // [2] tiles
+  uint8_t* kv_s = smem + 2 * C::kTile;  // [2] stages of K tile, V tile
+  uint64_t* bar = reinterpret_cast<uint64_t*>(kv_s + 4 * C::kTile);
+  uint64_t *q_full = bar, *s_full = bar + 2, *p_full = bar + 4, *o_full = bar + 6, *kv_full = bar + 8, *kv_empty = bar + 10;
+  uint64_t* mma_done = bar + 12;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 13);
+  __shared__ int s_fail;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    s_fail = 0;
+    for (int i = 0; i < 2; i++) {
+      ptx::mbar_init(&q_full[i], 128);
+      ptx::mbar_init(&s_full[i], 1);
+      ptx::mbar_init(&p_full[i], 128);
+      ptx::mbar_init(&o_full[i], 1);
+      ptx::mbar_init(&kv_full[i], kConvThreads);
+      ptx::mbar_init(&kv_empty[i], 1);
+    }
+    ptx::mbar_init(mma_done, 1);
+    ptx::fence_mbar_init();
+  }
+  if (warp == 12) ptx::tmem_alloc(tmem_slot, kTmem);
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_launch();
+
+  Item it;
+  int j0, j1, ns;
+  bool ok = true;
+  if (warp >= 8 && warp < 12) {
+    // ---- codes to values ------------------------------------------------------------------------
+    constexpr int P = D / 32;
+    const int tid = threadIdx.x - kSoftThreads;
+    uint32_t n = 0;  // key tiles converted so far, over all items
+    for (int idx = blockIdx.x; ok && find_item(p, BS, idx, it); idx += gridDim.x) {
+      span(p, it, j0, j1, ns);
+      if (j0 >= j1) continue;
+      Raw<D, NG> nxt;
+      load_raw<D, NG, BS>(nxt, p, it, j0, tid);
+      for (int j = j0; j < j1; j++, n++) {
+        const Raw<D, NG> r = nxt;
+        if (j + 1 < j1) load_raw<D, NG, BS>(nxt, p, it, j + 1, tid);
+        const int s = n & 1;
+        if (n >= 2) ok = __all_sync(0xffffffffu, ptx::mbar_wait(&kv_empty[s], ((n >> 1) - 1) & 1));
+        if (!ok) break;
+        uint8_t* kt = kv_s + s * 2 * C::kTile;
+#pragma unroll
+        for (int i = 0; i < P; i++) {
+          const int row = i * (kConvThreads / P) + tid / P;
+          store_piece<D, NG>(kt, row, tid % P, r.k[i], r.km[i]);
+          store_piece<D, NG>(kt + C::kTile, row, tid % P, r.v[i], r.vm[i]);
+        }
+        ptx::fence_proxy_async();
+        ptx::mbar_arrive(&kv_full[s]);
+      }
+    }
+    if (!ok) s_fail = 1;
+  } else if (warp == 12) {
+    // ---- MMA issuer -----------------------------------------------------------------------------
+    constexpr uint32_t idesc_s = ptx::idesc_bf16_f32(kRows, kKeys);
+    constexpr uint32_t idesc_o = ptx::idesc_bf16_f32_bmn(kRows, D);
+    uint32_t n = 0, items = 0;
+    auto qk = [&](int t, int s) {  // S_t = Q_t . K^T
+#pragma unroll
+      for (int kk = 0; kk < D / 16; kk++) {
+        const uint64_t a = ptx::sw128_kmajor_desc(ptx::smem_u32(q_s + t * C::kTile + (kk >> 2) * C::kChunk)) + 2 * (kk & 3);
+        const uint64_t b = ptx::sw128_kmajor_desc(ptx::smem_u32(kv_s + s * 2 * C::kTile + (kk >> 2) * C::kChunk)) + 2 * (kk & 3);
+        ptx::mma_f16_ss(tmem + t * 128, a, b, idesc_s, kk > 0 ? 1u : 0u);
+      }
+      ptx::mma_commit(&s_full[t]);
+    };
+    for (int idx = blockIdx.x; ok && find_item(p, BS, idx, it); idx += gridDim.x) {
+      span(p, it, j0, j1, ns);
+      if (j0 >= j1) continue;
+      if (lane == 0) {
+        ok = ptx::mbar_wait(&kv_full[n & 1], (n >> 1) & 1);
+        for (int t = 0; ok && t < 2; t++) {
+          ok = ptx::mbar_wait(&q_full[t], items & 1);
+          if (!ok) break;
+          ptx::tc_fence_after();
+          qk(t, n & 1);
+        }
+        for (int j = j0; ok && j < j1; j++, n++) {
+          const int s = n & 1;
+          const uint8_t* vt = kv_s + s * 2 * C::kTile + C::kTile;
+          for (int t = 0; ok && t < 2; t++) {
+            ok = ptx::mbar_wait(&p_full[t], n & 1);
+            if (!ok) break;
+            ptx::tc_fence_after();
+#pragma unroll
+            for (int kk = 0; kk < kKeys / 16; kk++)
+              ptx::mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8,
+                              ptx::sw128_mnmajor_desc(ptx::smem_u32(vt + kk * 16 * 128), C::kChunk), idesc_o,
+                              (j > j0 || kk > 0) ? 1u : 0u);
+            if (t == 1) ptx::mma_commit(&kv_empty[s]);
+            if (j + 1 < j1) {
+              if (t == 0) ok = ptx::mbar_wait(&kv_full[s ^ 1], ((n + 1) >> 1) & 1);
+              if (!ok) break;
+              ptx::tc_fence_after();
+              qk(t, s ^ 1);  // after P_t . V in the tensor core's order, which P_t's columns wait for
+            } else {
+              ptx::mma_commit(&o_full[t]);
+            }
+          }
+        }
+        items++;
+      }
+      ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+    }
+    if (lane == 0) {
+      if (!ok) s_fail = 1;
+      ptx::mma_commit(mma_done);  // nothing of this CTA is in flight past here
+      ptx::mbar_wait(mma_done, 0);
+    }
+  } else {
+    // ---- softmax --------------------------------------------------------------------------------
+    const int t = warp >> 2;
+    const int r = threadIdx.x & 127;  // row of the tile (TMEM lane)
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_t = tmem + t * 128 + lane_base, o_t = tmem + 256 + t * 128 + lane_base;
+    const int token = r / p.G, head = r - token * p.G;
+    const float c = p.scale_log2, slack = 8.f / c;
+    uint32_t n = 0, items = 0;
+    for (int idx = blockIdx.x; ok && find_item(p, BS, idx, it); idx += gridDim.x) {
+      span(p, it, j0, j1, ns);
+      const int tok0 = it.tile * 2 * p.tt + t * p.tt;  // the tile's first token of the sequence
+      const int at = tok0 + token;
+      const bool real = token < p.tt && at < it.rows;
+      const int64_t row = it.row0 + at;
+      const int pos = it.ctx - it.rows + at;
+      __nv_bfloat16* out = p.out + (row * p.hq + it.head * p.G + head) * (int64_t)D;
+      if (real && it.split == 0 && it.head == 0 && head == 0 && p.part_ns != nullptr) p.part_ns[row] = ns;
+      if (j0 >= j1) {
+        if (it.split == 0 && real)  // no key at all
+          for (int i = 0; i < D / 8; i++) reinterpret_cast<uint4*>(out)[i] = make_uint4(0, 0, 0, 0);
+        continue;
+      }
+      // the tile's query rows: 16-byte units in memory's order, swizzled (a row past the sequence: zeros)
+      for (int u = threadIdx.x & 127; u < 128 * (D / 8); u += 128) {
+        const int rr = u / (D / 8), k = u % (D / 8);
+        const int tk = rr / p.G, hh = rr - tk * p.G;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (tk < p.tt && tok0 + tk < it.rows)
+          v = *reinterpret_cast<const uint4*>(p.q + (int64_t)(it.row0 + tok0 + tk) * p.q_stride +
+                                              (int64_t)(it.head * p.G + hh) * D + 8 * k);
+        *reinterpret_cast<uint4*>(q_s + t * C::kTile + (k >> 3) * C::kChunk + rr * 128 + (((k & 7) ^ (rr & 7)) << 4)) = v;
+      }
+      ptx::fence_proxy_async();
+      ptx::mbar_arrive(&q_full[t]);
+
+      float m = -INFINITY, l = 0.f;
+      for (int j = j0; j < j1; j++, n++) {
+        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&s_full[t], n & 1));
+        if (!ok) break;
+        ptx::tc_fence_after();
+        const int key0 = j * kKeys;
+        const bool masked = __any_sync(0xffffffffu, key0 + kKeys - 1 > pos);
+        float mx = -INFINITY;
+        uint32_t v[32];
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          ptx::tmem_ld32(s_t + q * 32, v);
+          ptx::tmem_wait_ld();
+          if (masked) {
+#pragma unroll
+            for (int i = 0; i < 32; i++)
+              if (key0 + q * 32 + i <= pos) mx = fmaxf(mx, __uint_as_float(v[i]));
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; i++) mx = fmaxf(mx, __uint_as_float(v[i]));
+          }
+        }
+        if (__any_sync(0xffffffffu, mx > m + slack)) {
+          const float mn = fmaxf(m, mx);
+          const float a = m == -INFINITY ? 0.f : ex2((m - mn) * c);
+          m = mn;
+          l *= a;
+          if (j > j0) {
+#pragma unroll
+            for (int q = 0; q < D / 32; q++) {
+              ptx::tmem_ld32(o_t + q * 32, v);
+              ptx::tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * a);
+              ptx::tmem_st32(o_t + q * 32, v);
+            }
+          }
+        }
+        const float mc = m == -INFINITY ? 0.f : m * c;
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          ptx::tmem_ld32(s_t + q * 32, v);
+          ptx::tmem_wait_ld();
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            float a = ex2(fmaf(__uint_as_float(v[2 * i]), c, -mc)), b = ex2(fmaf(__uint_as_float(v[2 * i + 1]), c, -mc));
+            if (masked) {
+              if (key0 + q * 32 + 2 * i > pos) a = 0.f;
+              if (key0 + q * 32 + 2 * i + 1 > pos) b = 0.f;
+            }
+            l += a + b;
+            pk[i] = ptx::pack_bf16x2(a, b);
+          }
+          ptx::tmem_st16(s_t + q * 16, pk);  // P over the columns of S already read
+        }
+        ptx::tmem_wait_st();
+        ptx::tc_fence_before();
+        ptx::mbar_arrive(&p_full[t]);
+      }
+      if (ok) ok = __all_sync(0xffffffffu, ptx::mbar_wait(&o_full[t], items & 1));
+      if (!ok) break;
+      items++;
+      ptx::tc_fence_after();
+      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+      const int64_t part = (row * p.hq + it.head * p.G + head) * (int64_t)p.max_splits + it.split;
+#pragma unroll
+      for (int q = 0; q < D / 32; q++) {
+        uint32_t v[32];
+        ptx::tmem_ld32(o_t + q * 32, v);
+        ptx::tmem_wait_ld();
+        if (!real) continue;
+        if (ns == 1) {
+#pragma unroll
+          for (int u = 0; u < 4; u++) {
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) f[i] = l > 0.f || l != l ? __uint_as_float(v[u * 8 + i]) * inv : 0.f;
+            reinterpret_cast<uint4*>(out)[q * 4 + u] = pack8(f);
+          }
+        } else {
+#pragma unroll
+          for (int u = 0; u < 8; u++)
+            reinterpret_cast<uint4*>(p.part_o + part * D)[q * 8 + u] = make_uint4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+        }
+      }
+      if (real && ns > 1) p.part_ml[2 * part] = m * c, p.part_ml[2 * part + 1] = l;
+      ptx::tc_fence_before();
+    }
+    if (!ok) s_fail = 1;
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == 12) ptx::tmem_dealloc(tmem, kTmem);
+  if (threadIdx.x == 0 && s_fail && p.status) atomicExch(p.status, (int)kTimeout);
+}
+
+// Rows cut along their keys: out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i, in order. A warp per
+// (row, query head).
+template <int D>
+__global__ void __launch_bounds__(128) prefill_merge_kernel(PreParams p) {
+  constexpr int E = D / 32;
+  pdl_wait();
+  pdl_launch();
+  const int64_t rh = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (rh >= (int64_t)p.T * p.hq) return;
+  const int ns = min(p.part_ns[rh / p.hq], p.max_splits);
+  if (ns <= 1) return;
+  const float* ml = p.part_ml + rh * p.max_splits * 2;
+  float mx = -INFINITY;
+  for (int i = lane; i < ns; i += 32) mx = fmaxf(mx, ml[2 * i]);
+  mx = warp_max(mx);
+  float acc[E], l = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; e++) acc[e] = 0.f;
+  for (int i = 0; i < ns; i++) {
+    const float mi = ml[2 * i];
+    const float f = mi == mx ? 1.f : ex2(mi - mx);
+    l = fmaf(ml[2 * i + 1], f, l);
+    const float* po = p.part_o + (rh * p.max_splits + i) * D;
+#pragma unroll
+    for (int e = 0; e < E; e++) acc[e] = fmaf(po[e * 32 + lane], f, acc[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < E; e++) p.out[rh * D + e * 32 + lane] = f2bf(l > 0.f || l != l ? acc[e] / l : 0.f);
+}
+
+template <int D, int NG, int BS>
+cudaError_t launch_prefill(const PreParams& p, int grid, cudaStream_t stream) {
+  static std::atomic<uint64_t> configured{0};
+  cudaError_t e = once_per_device(configured, [] {
+    return cudaFuncSetAttribute(prefill_kernel<D, NG, BS>, cudaFuncAttributeMaxDynamicSharedMemorySize, PreCfg<D>::kSmem);
+  });
+  if (e != cudaSuccess) return e;
+  e = launch_ex(prefill_kernel<D, NG, BS>, dim3(grid), dim3(kPreThreads), PreCfg<D>::kSmem, stream, 0, p);
+  if (e != cudaSuccess || p.max_splits == 1) return e;
+  return launch_ex(prefill_merge_kernel<D>, dim3((unsigned)(((int64_t)p.T * p.hq + 3) / 4)), dim3(128), 0, stream, 0, p);
+}
+
+}  // namespace kv4
+
+int64_t kv4_prefill_splits(int64_t T, int64_t S, int64_t hq, int64_t hkv, int64_t max_len) {
+  if (T <= 0 || S <= 0 || hkv <= 0 || hq < hkv || hq / hkv > kv4::kRows) return 1;
+  const int64_t J = (max_len + kv4::kKeys - 1) / kv4::kKeys;
+  const int64_t tt2 = 2 * (kv4::kRows / (hq / hkv));
+  // one sequence: its rows are the step's; several: one of them may have as few as one
+  const int chunk = kv4::chunk_of(S == 1 ? (int)((T + tt2 - 1) / tt2) : 1, (int)hkv);
+  return J <= chunk ? 1 : (J + chunk - 1) / chunk;
+}
+
+cudaError_t launch_kv4_prefill(const Kv4PrefillArgs& a, cudaStream_t stream) {
+  if (a.T == 0 || a.S == 0) return cudaSuccess;
+  if (a.c.hkv <= 0 || a.hq % a.c.hkv != 0 || a.hq / a.c.hkv > kv4::kRows || a.max_splits < 1 || !(a.scale > 0.f))
+    return cudaErrorInvalidValue;
+  if (a.T > INT32_MAX / 2 || a.bt_cols * a.c.block_size > INT32_MAX - kv4::kKeys || a.T * a.hq > ((int64_t)1 << 32))
+    return cudaErrorInvalidValue;
+  kv4::PreParams p{};
+  p.q = static_cast<const __nv_bfloat16*>(a.q);
+  p.q_stride = a.q_stride;
+  p.cache = static_cast<const uint8_t*>(a.c.base);
+  p.s_block = a.c.s_block;
+  p.num_blocks = a.c.num_blocks;
+  p.block_tables = a.block_tables;
+  p.bt_stride = a.bt_stride;
+  p.bt_cols = (int)a.bt_cols;
+  p.ctx_lens = a.ctx_lens;
+  p.last_rows = a.last_rows;
+  p.out = static_cast<__nv_bfloat16*>(a.out);
+  p.part_o = a.part_o;
+  p.part_ml = a.part_ml;
+  p.part_ns = a.max_splits > 1 ? a.part_ns : nullptr;
+  p.status = a.status;
+  p.T = (int)a.T;
+  p.S = (int)a.S;
+  p.hq = a.hq;
+  p.hkv = a.c.hkv;
+  p.G = a.hq / a.c.hkv;
+  p.tt = kv4::kRows / p.G;
+  p.max_splits = a.max_splits;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  // items: at most a row tile per 2 tt rows and sequence, each times heads and splits
+  const int64_t most = (a.T / (2 * p.tt) + a.S) * p.hkv * a.max_splits;
+  const int grid = (int)(most < a.num_sms ? most : a.num_sms);
+  return kv4::pick(a.c.d, a.c.groups, a.c.block_size, [&](auto d, auto ng, auto bs) {
+    return kv4::launch_prefill<d, ng, bs>(p, grid, stream);
+  });
+}
+
+}  // namespace es

@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <atomic>
 #include <chrono>
 #include <cstring>
@@ -713,11 +714,10 @@ void on_device_of(const torch::Tensor& t, at::ScalarType st, const torch::Tensor
   TORCH_CHECK(t.is_cuda() && t.device() == peer.device() && t.scalar_type() == st, what);
 }
 
-void rope_kv4_write(torch::Tensor qkv, c10::optional<torch::Tensor> bias, torch::Tensor positions,
-                    torch::Tensor cos_sin, torch::Tensor slots, torch::Tensor q_out, torch::Tensor cache, int64_t hq,
-                    int64_t hkv, int64_t block_size, torch::Tensor status) {
+torch::Tensor rope_kv4_write(torch::Tensor qkv, c10::optional<torch::Tensor> bias, torch::Tensor positions,
+                             torch::Tensor cos_sin, torch::Tensor slots, torch::Tensor cache, int64_t hq, int64_t hkv,
+                             int64_t block_size, torch::Tensor status) {
   check_bf16(qkv, "qkv");
-  check_bf16(q_out, "q_out");
   on_device_of(cos_sin, at::kFloat, qkv, "cos_sin: fp32 [positions, head_dim] on the device of qkv");
   TORCH_CHECK(cos_sin.dim() == 2 && cos_sin.is_contiguous() && cos_sin.size(0) > 0 &&
                   reinterpret_cast<uintptr_t>(cos_sin.data_ptr()) % 16 == 0,
@@ -736,7 +736,6 @@ void rope_kv4_write(torch::Tensor qkv, c10::optional<torch::Tensor> bias, torch:
   TORCH_CHECK(positions.dim() == 1 && positions.is_contiguous() && positions.numel() >= T && slots.dim() == 1 &&
                   slots.is_contiguous() && slots.numel() >= T,
               "positions and slots: one contiguous value per row");
-  TORCH_CHECK(q_out.device() == qkv.device() && q_out.is_contiguous() && q_out.numel() == T * hq * d, "q_out must be [T, hq, head_dim]");
   if (bias.has_value()) {
     check_bf16(*bias, "bias");
     TORCH_CHECK(bias->device() == qkv.device() && bias->is_contiguous() && bias->numel() == qkv.size(1) &&
@@ -751,83 +750,130 @@ void rope_kv4_write(torch::Tensor qkv, c10::optional<torch::Tensor> bias, torch:
   a.cos_sin = cos_sin.data_ptr<float>();
   a.max_pos = cos_sin.size(0);
   a.slots = slots.data_ptr<int64_t>();
-  a.q_out = q_out.data_ptr();
   a.T = T;
   a.hq = (int)hq;
   a.status = status.data_ptr<int>();
   const c10::cuda::CUDAGuard g(qkv.device());
+  torch::Tensor q_out = torch::empty({T, hq, d}, qkv.options());
+  a.q_out = q_out.data_ptr();
   ES_CHECK_CUDA(es::launch_rope_kv4(a, cur()));
+  return q_out;
 }
 
-void kv4_read(torch::Tensor cache, torch::Tensor slots, torch::Tensor k, torch::Tensor v, int64_t d,
-              int64_t block_size, torch::Tensor status) {
-  check_bf16(k, "k");
-  check_bf16(v, "v");
+std::tuple<torch::Tensor, torch::Tensor> kv4_read(torch::Tensor cache, torch::Tensor slots, int64_t d,
+                                                  int64_t block_size, torch::Tensor status) {
   es::Kv4ReadArgs a{};
-  a.c = kv4_cache(cache, d, block_size, k);
+  a.c = kv4_cache(cache, d, block_size, cache);
   on_device_of(slots, at::kLong, cache, "slots: int64 on the device of the cache");
   TORCH_CHECK(slots.dim() == 1 && slots.is_contiguous(), "slots: one contiguous value per row");
   const int64_t n = slots.numel();
-  TORCH_CHECK(k.is_contiguous() && v.is_contiguous() && v.device() == k.device() && k.numel() == n * a.c.hkv * d &&
-                  v.numel() == k.numel(),
-              "k and v must be [n, kv_heads, head_dim]");
   on_device_of(status, at::kInt, cache, "status must be int32 on the device of the cache");
   a.slots = slots.data_ptr<int64_t>();
-  a.k = k.data_ptr();
-  a.v = v.data_ptr();
   a.n = n;
   a.status = status.data_ptr<int>();
   const c10::cuda::CUDAGuard g(cache.device());
+  torch::Tensor k = torch::empty({n, a.c.hkv, d}, cache.options().dtype(at::kBFloat16)), v = torch::empty_like(k);
+  a.k = k.data_ptr();
+  a.v = v.data_ptr();
   ES_CHECK_CUDA(es::launch_kv4_read(a, cur()));
+  return {k, v};
 }
 
-void paged_decode_kv4(torch::Tensor q, torch::Tensor cache, torch::Tensor block_tables, torch::Tensor ctx_lens,
-                      torch::Tensor out, torch::Tensor part_o, torch::Tensor part_ml, torch::Tensor status,
-                      int64_t block_size, int64_t max_splits, double scale) {
-  check_bf16(q, "q");
-  check_bf16(out, "out");
-  TORCH_CHECK(q.dim() == 3, "q must be [B, hq, head_dim]");
-  const int64_t B = q.size(0), hq = q.size(1), d = q.size(2);
-  es::Kv4DecodeArgs a{};
-  a.c = kv4_cache(cache, d, block_size, q);
-  TORCH_CHECK(hq >= 1 && hq % a.c.hkv == 0, "query heads must be a multiple of the cache's kv heads");
+// The checks that decode and prefill share: q [rows, hq, d], int32 block tables [seqs, blocks], int32
+// ctx_lens [seqs].
+es::Kv4Cache kv4_attention_args(const torch::Tensor& q, const torch::Tensor& cache, const torch::Tensor& block_tables,
+                                const torch::Tensor& ctx_lens, const torch::Tensor& status, int64_t seqs,
+                                int64_t block_size) {
+  const es::Kv4Cache c = kv4_cache(cache, q.size(2), block_size, q);
+  const int64_t rows = q.size(0), hq = q.size(1), d = q.size(2);
+  TORCH_CHECK(hq >= 1 && hq % c.hkv == 0, "query heads must be a multiple of the cache's kv heads");
   TORCH_CHECK(q.stride(2) == 1 && (hq == 1 || q.stride(1) == d) &&
-                  (B <= 1 || (q.stride(0) % 8 == 0 && q.stride(0) >= hq * d)) &&
+                  (rows <= 1 || (q.stride(0) % 8 == 0 && q.stride(0) >= hq * d)) &&
                   reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0,
               "q rows must be contiguous and 16-byte aligned");
-  TORCH_CHECK(out.device() == q.device() && out.is_contiguous() && out.sizes() == q.sizes() &&
-                  reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0,
-              "out must be [B, hq, head_dim]");
   on_device_of(block_tables, at::kInt, q, "block_tables: int32 on the device of q");
   on_device_of(ctx_lens, at::kInt, q, "ctx_lens: int32 on the device of q");
-  TORCH_CHECK(block_tables.dim() == 2 && block_tables.stride(1) == 1 && block_tables.size(0) >= B &&
-                  ctx_lens.dim() == 1 && ctx_lens.is_contiguous() && ctx_lens.numel() >= B,
-              "block_tables [B, blocks] and ctx_lens [B], rows contiguous");
-  TORCH_CHECK(B == 0 || (a.c.num_blocks > 0 && block_tables.size(1) > 0), "an empty cache or block table");
-  on_device_of(part_o, at::kFloat, q, "part_o: fp32 on the device of q");
-  on_device_of(part_ml, at::kFloat, q, "part_ml: fp32 on the device of q");
-  TORCH_CHECK(max_splits >= 1 && max_splits <= INT32_MAX &&
-                  (max_splits == 1 || (part_o.is_contiguous() && part_ml.is_contiguous() &&
-                                       part_o.numel() >= B * hq * max_splits * d &&
-                                       part_ml.numel() >= B * hq * max_splits * 2)),
-              "split scratch too small");
+  TORCH_CHECK(block_tables.dim() == 2 && block_tables.stride(1) == 1 && block_tables.size(0) >= seqs &&
+                  ctx_lens.dim() == 1 && ctx_lens.is_contiguous() && ctx_lens.numel() >= seqs,
+              "block_tables [sequences, blocks] and ctx_lens [sequences], rows contiguous");
+  TORCH_CHECK(seqs == 0 || (c.num_blocks > 0 && block_tables.size(1) > 0), "an empty cache or block table");
   on_device_of(status, at::kInt, q, "status must be int32 on the device of q");
+  return c;
+}
+
+torch::Tensor paged_decode_kv4(torch::Tensor q, torch::Tensor cache, torch::Tensor block_tables,
+                               torch::Tensor ctx_lens, torch::Tensor status, int64_t block_size, int64_t max_model_len,
+                               double scale) {
+  check_bf16(q, "q");
+  TORCH_CHECK(q.dim() == 3, "q must be [B, hq, head_dim]");
+  TORCH_CHECK(max_model_len >= 1, "max_model_len must be positive");
+  const int64_t B = q.size(0), hq = q.size(1), d = q.size(2);
+  es::Kv4DecodeArgs a{};
+  a.c = kv4_attention_args(q, cache, block_tables, ctx_lens, status, B, block_size);
   a.q = q.data_ptr();
   a.q_stride = q.stride(0);
   a.block_tables = block_tables.data_ptr<int>();
   a.bt_stride = block_tables.stride(0);
   a.bt_cols = block_tables.size(1);
   a.ctx_lens = ctx_lens.data_ptr<int>();
-  a.out = out.data_ptr();
-  a.part_o = part_o.data_ptr<float>();
-  a.part_ml = part_ml.data_ptr<float>();
   a.status = status.data_ptr<int>();
   a.B = (int)B;
   a.hq = (int)hq;
-  a.max_splits = (int)max_splits;
   a.scale = (float)scale;
   const c10::cuda::CUDAGuard g(q.device());
+  torch::Tensor out = torch::empty({B, hq, d}, q.options()), part;
+  a.out = out.data_ptr();
+  const int64_t splits = es::kv4_max_splits(max_model_len);
+  a.max_splits = (int)splits;
+  if (splits > 1) {
+    part = torch::empty({B * hq * splits * (d + 2)}, q.options().dtype(at::kFloat));
+    a.part_o = part.data_ptr<float>();
+    a.part_ml = a.part_o + B * hq * splits * d;
+  }
   ES_CHECK_CUDA(es::launch_kv4_decode(a, cur()));
+  return out;
+}
+
+torch::Tensor paged_prefill_kv4(torch::Tensor q, torch::Tensor cache, torch::Tensor block_tables,
+                                torch::Tensor ctx_lens, torch::Tensor last_rows, torch::Tensor status,
+                                int64_t block_size, int64_t max_context, double scale, int64_t num_sms) {
+  check_bf16(q, "q");
+  TORCH_CHECK(q.dim() == 3, "q must be [T, hq, head_dim]");
+  on_device_of(last_rows, at::kLong, q, "last_rows: int64 on the device of q");
+  TORCH_CHECK(last_rows.dim() == 1 && last_rows.is_contiguous(), "last_rows: one contiguous value per sequence");
+  TORCH_CHECK(scale > 0, "scale must be positive");
+  TORCH_CHECK(max_context >= 1 && num_sms >= 1, "max_context and num_sms must be positive");
+  const int64_t T = q.size(0), S = last_rows.numel(), hq = q.size(1), d = q.size(2);
+  es::Kv4PrefillArgs a{};
+  a.c = kv4_attention_args(q, cache, block_tables, ctx_lens, status, S, block_size);
+  TORCH_CHECK(hq / a.c.hkv <= 128, "at most 128 query heads to a kv head");
+  a.q = q.data_ptr();
+  a.q_stride = q.stride(0);
+  a.block_tables = block_tables.data_ptr<int>();
+  a.bt_stride = block_tables.stride(0);
+  a.bt_cols = block_tables.size(1);
+  a.ctx_lens = ctx_lens.data_ptr<int>();
+  a.last_rows = last_rows.data_ptr<int64_t>();
+  a.status = status.data_ptr<int>();
+  a.T = T;
+  a.S = S;
+  a.hq = (int)hq;
+  a.num_sms = (int)num_sms;
+  a.scale = (float)scale;
+  const c10::cuda::CUDAGuard g(q.device());
+  torch::Tensor out = torch::empty({T, hq, d}, q.options()), part;
+  a.out = out.data_ptr();
+  const int64_t splits =
+      es::kv4_prefill_splits(T, S, hq, a.c.hkv, std::min<int64_t>(max_context, block_tables.size(1) * block_size));
+  a.max_splits = (int)splits;
+  if (splits > 1) {
+    part = torch::empty({T * hq * splits * (d + 2) + T}, q.options().dtype(at::kFloat));
+    a.part_o = part.data_ptr<float>();
+    a.part_ml = a.part_o + T * hq * splits * d;
+    a.part_ns = reinterpret_cast<int*>(a.part_ml + T * hq * splits * 2);
+  }
+  ES_CHECK_CUDA(es::launch_kv4_prefill(a, cur()));
+  return out;
 }
 
 // caches[l][pairs[i, 1]] = caches[l][pairs[i, 0]]: pages are the first dimension, contiguous inside
@@ -1068,7 +1114,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rope_kv4_write", &rope_kv4_write, "RoPE on q/k and the write of k/v into the paged cache held in 4 bits");
   m.def("kv4_read", &kv4_read, "values of rows of the paged cache held in 4 bits");
   m.def("paged_decode_kv4", &paged_decode_kv4, "decode attention over the paged cache held in 4 bits");
-  m.def("kv4_max_splits", &es::kv4_max_splits, "splits of a history of at most max_len positions");
+  m.def("paged_prefill_kv4", &paged_prefill_kv4, "causal prefill attention over the paged cache held in 4 bits (tcgen05)");
   m.def("copy_pages", &copy_pages, "pages copied in every layer's cache, one launch");
   m.def("moe_route", &moe_route, "mixture routing: per-token weights of this rank's experts [el, T]");
   m.def("moe_topk", &moe_topk, "mixture routing: each token's top k experts and their weights");

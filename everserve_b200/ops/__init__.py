@@ -74,7 +74,7 @@ class RefOps:
         rows = torch.arange(q.shape[0], device=q.device)
         return ref.kv4_attention(q, cache, block_tables, ctx_lens[: q.shape[0]], rows, scale, block_size)
 
-    def prefill_attention_kv4(self, q, cache, block_tables, ctx_lens, last_rows, scale, block_size):
+    def prefill_attention_kv4(self, q, cache, block_tables, ctx_lens, last_rows, scale, block_size, max_context=None):
         return ref.kv4_attention(q, cache, block_tables, ctx_lens, last_rows, scale, block_size)
 
     def copy_pages(self, caches, pairs):
@@ -272,30 +272,30 @@ class KernelOps:
         """RoPE on q and k, k and v quantised to 4 bits into their slots of `cache` (uint8, of
         ``ref.kv4_cache_shape``); returns q [T, hq, d]. A negative slot is not written; a position or
         slot out of range is reported by ``check_status``."""
-        q = torch.empty(qkv.shape[0], hq, cos_sin.shape[1], dtype=qkv.dtype, device=qkv.device)
-        self.C.rope_kv4_write(qkv, bias, positions, cos_sin, slots, q, cache, hq, hkv, block_size, self.status)
-        return q
+        return self.C.rope_kv4_write(qkv, bias, positions, cos_sin, slots, cache, hq, hkv, block_size, self.status)
 
     def kv4_read(self, cache, slots, head_dim, block_size):
         """The rows at `slots` (int64 [n]) as bf16 k, v [n, kv_heads, head_dim]; zeros for a negative slot."""
-        kv = torch.empty(2, slots.shape[0], cache.shape[1], head_dim, dtype=torch.bfloat16, device=cache.device)
-        self.C.kv4_read(cache, slots, kv[0], kv[1], head_dim, block_size, self.status)
-        return kv[0], kv[1]
+        return self.C.kv4_read(cache, slots, head_dim, block_size, self.status)
 
     def decode_attention_kv4(self, q, cache, block_tables, ctx_lens, scale, block_size, max_model_len=None):
         """Attention of one query row per sequence over its history in 4 bits: q [B, hq, d] -> [B, hq, d];
         an empty history gives zeros. The result of a sequence does not depend on its batch. The
         workspace is the call's own, so calls on several streams do not meet in it."""
-        B, hq, d = q.shape
         if max_model_len is None:
             max_model_len = block_tables.shape[1] * block_size
-        ms = int(self.C.kv4_max_splits(max_model_len))
-        out = torch.empty(B, hq, d, dtype=q.dtype, device=q.device)
-        part = torch.empty(B * hq * ms * (d + 2) if ms > 1 else 0, dtype=torch.float32, device=q.device)
-        n = B * hq * ms * d if ms > 1 else 0
-        self.C.paged_decode_kv4(q, cache, block_tables, ctx_lens, out, part[:n], part[n:], self.status, block_size, ms,
-                                scale)
-        return out
+        return self.C.paged_decode_kv4(q, cache, block_tables, ctx_lens, self.status, block_size, max_model_len, scale)
+
+    def prefill_attention_kv4(self, q, cache, block_tables, ctx_lens, last_rows, scale, block_size, max_context=None):
+        """Causal attention of a step's new rows over their sequences' history in 4 bits (the rows' own
+        keys and values written before): sequence s owns the rows up to last_rows[s] (int64, on the
+        device), the last of them at position ctx_lens[s] - 1. q [T, hq, d] -> [T, hq, d]; a row without a
+        visible key gives zeros. `max_context` bounds the step's context lengths (default: what
+        block_tables can hold); it sizes the call's own workspace, nothing else."""
+        if max_context is None:
+            max_context = block_tables.shape[1] * block_size
+        return self.C.paged_prefill_kv4(q, cache, block_tables, ctx_lens, last_rows, self.status, block_size,
+                                        max_context, scale, self.num_sms)
 
     def copy_pages(self, caches, pairs):
         """Copy pages (the first dimension's entries) in every layer's cache, bf16 or 4-bit: pairs int64

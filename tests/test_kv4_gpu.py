@@ -3,7 +3,9 @@
 Writes are held to the format's formula byte for byte (each of its operations is one IEEE rounding).
 Attention is held, value by value, to what its roundings allow: with o the exact output and A = sum_t p_t
 max_d |v_td|, the bf16 result is within 2^-9 |o| (its own rounding), P * scale in f16 and the code sums
-within 2^-10 A, P in bf16 (prefill) within 2^-8 A with its V and K values in bf16; one bit is allowed on top.
+within 2^-10 A; prefill's P and V in bf16 within 2^-8 A, and its K in bf16 moves a score by noise of deviation
+scale 2^-9 sqrt(sum_d (q_d k_td)^2 / 3), of which six are allowed, taken at the worst key. One bit is allowed
+on top of the f16 figure.
 """
 
 import math
@@ -274,6 +276,75 @@ def test_copy_pages(kops, kind, layers, n, hkv, d, bs):
     kops.copy_pages(caches, pairs[:0])
 
 
+def prefill_mag(q, cache, tables, lens, last, scale, bs):
+    """2^-8 and six deviations of a score's noise, per row and head."""
+    hq, d = q.shape[1:]
+    vals = ref.kv4_cache_values(cache, d, bs).double()
+    out = torch.zeros(q.shape[0], hq, 1, dtype=torch.float64, device="cuda")
+    r0 = 0
+    for s, (r1, n) in enumerate(zip((last + 1).tolist(), lens.tolist())):
+        if n:
+            k = vals[tables[s, : -(-n // bs)].long(), 0].transpose(1, 2).reshape(-1, cache.shape[1], d)[:n]
+            sq = torch.einsum("thd,nhd->thn", q[r0:r1].double() ** 2, k.repeat_interleave(hq // cache.shape[1], 1) ** 2)
+            out[r0:r1] = sq.amax(-1, keepdim=True)
+        r0 = r1
+    return 2.0**-8 + 6 * 2.0**-9 * scale * (out / 3).sqrt()
+
+
+@pytest.mark.parametrize("hq,hkv,d,group,bs", LAYOUTS)
+def test_prefill(kops, hq, hkv, d, group, bs):
+    """Rows from one to several tiles, histories from none to long (cut along the keys), ends inside tiles
+    and blocks, a sequence without keys, one with more rows than keys."""
+    rows = [1, 2, 31, 64, 127, 128, 129, 300, 1, 5, 33, 70, 1, 9, 600]
+    past = [0, 0, 0, 0, 1, 0, 15, 0, 700, 1027, 2300, 5000, -1, -4, 200]
+    lens = [r + p for r, p in zip(rows, past)]
+    q, cache, tables, ctx, last = batch(lens, rows, hq, hkv, d, group, bs, 31)
+    scale = d**-0.5
+    out = kops.prefill_attention_kv4(q, cache, tables, ctx, last, scale, bs)
+    assert kops.check_status() == 0
+    want, mag = oracle(q, cache, tables, ctx, last, scale, bs)
+    held_to(out, want, mag, prefill_mag(q, cache, tables, ctx, last, scale, bs))
+    at = sum(rows[:13])
+    assert not bool(out[at : at + 4].any()) and not bool(out[at - 1].any())  # no visible key
+    assert torch.equal(out, kops.prefill_attention_kv4(q, cache, tables, ctx, last, scale, bs))
+    # a sequence alone gives the same bits
+    for s in (4, 7, 11):
+        r0 = sum(rows[:s])
+        one = kops.prefill_attention_kv4(q[r0 : r0 + rows[s]], cache, tables[s : s + 1], ctx[s : s + 1],
+                                         last[s : s + 1] - r0, scale, bs)
+        assert torch.equal(one, out[r0 : r0 + rows[s]])
+
+
+def test_prefill_many_sequences_and_long(kops):
+    """More sequences than a warp scans at once, and a prompt of several thousand rows."""
+    hq, hkv, d, group, bs = 8, 2, 128, 64, 16
+    rows = [1 + i % 5 for i in range(70)]
+    lens = [r + 7 * i for i, r in enumerate(rows)]
+    q, cache, tables, ctx, last = batch(lens, rows, hq, hkv, d, group, bs, 32)
+    out = kops.prefill_attention_kv4(q, cache, tables, ctx, last, 0.1, bs)
+    want, mag = oracle(q, cache, tables, ctx, last, 0.1, bs)
+    held_to(out, want, mag, prefill_mag(q, cache, tables, ctx, last, 0.1, bs))
+    q, cache, tables, ctx, last = batch([5003], [5003], hq, hkv, d, group, bs, 33)
+    out = kops.prefill_attention_kv4(q, cache, tables, ctx, last, 0.1, bs)
+    want, mag = oracle(q, cache, tables, ctx, last, 0.1, bs)
+    held_to(out, want, mag, prefill_mag(q, cache, tables, ctx, last, 0.1, bs))
+    assert kops.check_status() == 0
+
+
+def test_prefill_extremes(kops):
+    """Maxima that move late and far (the output is rescaled), and scores equal to the last bit."""
+    hq, hkv, d, group, bs = 4, 1, 128, 128, 16
+    q, cache, tables, ctx, last = batch([1500, 400], [300, 400], hq, hkv, d, group, bs, 34)
+    kp = ref.kv4_parts(cache, d, bs)[2].view(torch.bfloat16)
+    for key in (200, 900, 1290):
+        kp[tables[0, key // bs].long(), :, key % bs] *= 12
+    q[300:] = 0  # every key alike
+    out = kops.prefill_attention_kv4(q, cache, tables, ctx, last, d**-0.5, bs)
+    want, mag = oracle(q, cache, tables, ctx, last, d**-0.5, bs)
+    held_to(out, want, mag, prefill_mag(q, cache, tables, ctx, last, d**-0.5, bs))
+    assert kops.check_status() == 0
+
+
 def test_other_stream_and_graph(kops):
     """A call on a side stream, and a captured one replayed on new lengths and contents."""
     hq, hkv, d, group, bs = 32, 8, 128, 64, 16
@@ -325,6 +396,11 @@ def test_refusals(kops):
             kops.rope_kv4_write(a["qkv"], a["bias"], a["pos"], a["cs"], a["slots"], cache, hq, a["hkv"], bs)
     with pytest.raises(RuntimeError):
         kops.kv4_read(cache, i.int(), d, bs)
+    for bad in (dict(last=i.int()), dict(last=torch.cat([i, i])), dict(scale=0.0), dict(q=q.float())):
+        a = dict(q=q, last=i, scale=0.1)
+        a.update(bad)
+        with pytest.raises(RuntimeError):
+            kops.prefill_attention_kv4(a["q"], cache, bt, ctx, a["last"], a["scale"], bs)
     for caches, pairs in (([cache, cache[:2]], torch.zeros(1, 2, dtype=torch.int64, device=dev)),
                           ([cache[:, :, 16:32]], torch.zeros(1, 2, dtype=torch.int64, device=dev)),
                           ([cache], torch.zeros(1, 2, dtype=torch.int32, device=dev)),
