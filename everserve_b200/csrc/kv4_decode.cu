@@ -11,9 +11,10 @@
 //
 // S^T = K . q^T and O^T = V^T . P^T on mma.sync m16n8k16 (f16, fp32 sums): 16 keys by 8 query heads
 // of one kv head, so a group of 8 heads fills the tile. A query row is scaled to at most 2^10 by a power
-// of two, which keeps its bf16 values exact in f16 down to 2^-24. P_t scale_tg is rounded to f16 (11
-// bits) under a power of two that follows the largest scale seen; scores, sums, the zeros' part and
-// the output stay in fp32.
+// of two, which keeps its bf16 values exact in f16 down to 2^-24. The zeros' part of the scores is one
+// m16n8k8 on the bf16 zeros as stored, against sum q split into three bf16 terms (24 bits). P_t scale_tg
+// is rounded to f16 (11 bits) under a power of two that follows the largest scale seen; scores, sums, the
+// zeros' part and the output stay in fp32.
 //
 // A warp takes one (sequence, kv head, split of the history) by itself: the records of its blocks stream
 // through a ring of its own in shared memory, one bulk copy a block, and nothing but that ring's barriers
@@ -33,9 +34,10 @@ namespace kv4 {
 
 constexpr int kDecWarps = 4;
 constexpr int kDecThreads = kDecWarps * 32;
+constexpr int kDecCtas = 4;  // a SM
 constexpr float kLog2eF = 1.4426950408889634f;
 constexpr float kSlack = 6.f;       // log2 of how far a score may pass the running maximum
-constexpr float kPBits = 7.f;       // P * scale enters f16 as at most 2^(6 + 2 + 7) = 2^15
+constexpr int kPBits = 7;           // P * scale enters f16 as at most 2^(6 + 2 + 7) = 2^15
 
 // Keys of a split: short where a lone sequence needs the warps, longer where the ends of a split (query
 // in, partial result out) would cost more than they bring. At most 32 blocks, whose table entries a warp
@@ -46,10 +48,12 @@ __host__ __device__ __forceinline__ int splits_of(int n) { return n <= 128 ? 1 :
 
 template <int D, int NG, int BS>
 struct Ring {
-  // stages of a record each: 9 KB and more a warp, so that four CTAs of an SM keep over 100 KB on the way
-  static constexpr int kStages = Rec<D, NG, BS>::kBytes > 4096 ? 3 : 9216 / Rec<D, NG, BS>::kBytes;
+  // stages of a record each, about 14 KB a warp (an even count, as a step of 32 keys may take two)
+  static constexpr int kStages = Rec<D, NG, BS>::kBytes > 4096 ? 3 : 13824 / Rec<D, NG, BS>::kBytes / 2 * 2;
   static constexpr int kBytes = kStages * Rec<D, NG, BS>::kBytes;
-  static constexpr int kSmem = kDecWarps * (kBytes + 8 * kStages);
+  static constexpr int kStep = 32 / BS;                 // blocks of a step of 32 keys, which share a barrier
+  static constexpr int kSteps = kStages / kStep;
+  static constexpr int kSmem = kDecWarps * (kBytes + 8 * kSteps);
 };
 
 struct DecodeParams {
@@ -77,6 +81,13 @@ ES_DEVICE void mma_f16_16816(float* d, const uint32_t* a, uint32_t b0, uint32_t 
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// D (16x8 fp32) = A (16x8 bf16, row) * B (8x8 bf16, col) + C, C the same in every row
+ES_DEVICE void mma_bf16_1688(float* d, uint32_t a0, uint32_t a1, uint32_t b, float c0, float c1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%8,%7,%8};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(b), "f"(c0), "f"(c1));
+}
 // transpose of an 8 x 8 matrix of 16-bit values held two a lane
 ES_DEVICE uint32_t transpose8(uint32_t a) {
   uint32_t d;
@@ -96,176 +107,205 @@ ES_DEVICE int exponent(float x) { return min(90, max(-90, (int)((__float_as_uint
 // keys i and (i ^ 1) + 4, so that the eight lanes of a 16-byte shared load meet both halves of the banks.
 ES_DEVICE int key_of_row(int r) { return (r & 8) + ((r & 1) ? ((r >> 1 & 3) ^ 1) + 4 : (r >> 1 & 3)); }
 
-// What a lane (gid = lane / 4, tig = lane % 4) holds of a run of 16 keys.
-template <int D, int NG>
-struct Run {
-  uint32_t k[2][D / 32];          // K words of rows gid and gid + 8
-  uint32_t v[4][D / 64];          // V words of rows 2 tig, 2 tig + 1, 2 tig + 8, 2 tig + 9
-  uint32_t kp[2][NG], vp[2][NG];  // (scale, zero) pairs of rows gid and gid + 8
-};
-
-template <int D, int NG, int BS>
-ES_DEVICE void load_run(Run<D, NG>& r, const uint8_t* rec, int sub, int gid, int tig) {
-  using R = Rec<D, NG, BS>;
-#pragma unroll
-  for (int i = 0; i < 2; i++) {
-    const int row = sub * 16 + 8 * i + key_of_row(gid);
-    const uint8_t* kp = rec + row * R::kRow + tig * (D / 8);
-    if (D == 128) {
-      const uint4 w = *reinterpret_cast<const uint4*>(kp);
-      r.k[i][0] = w.x, r.k[i][1] = w.y, r.k[i][D / 32 - 2] = w.z, r.k[i][D / 32 - 1] = w.w;
-    } else {
-      const uint2 w = *reinterpret_cast<const uint2*>(kp);
-      r.k[i][0] = w.x, r.k[i][1] = w.y;
-    }
-    const uint8_t* mp = rec + R::kKMeta + row * R::kMeta;
-    if (NG == 2) {
-      const uint2 a = *reinterpret_cast<const uint2*>(mp);
-      const uint2 b = *reinterpret_cast<const uint2*>(mp + BS * R::kMeta);
-      r.kp[i][0] = a.x, r.kp[i][NG - 1] = a.y, r.vp[i][0] = b.x, r.vp[i][NG - 1] = b.y;
-    } else {
-      r.kp[i][0] = *reinterpret_cast<const uint32_t*>(mp);
-      r.vp[i][0] = *reinterpret_cast<const uint32_t*>(mp + BS * R::kMeta);
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < 4; j++) {
-    const int row = sub * 16 + 8 * (j >> 1) + ((j & 1) ? (tig ^ 1) + 4 : tig);
-    const uint8_t* vp = rec + R::kV + row * R::kRow + gid * (D / 16);
-    if (D == 128) {
-      const uint2 w = *reinterpret_cast<const uint2*>(vp);
-      r.v[j][0] = w.x, r.v[j][D / 64 - 1] = w.y;
-    } else {
-      r.v[j][0] = *reinterpret_cast<const uint32_t*>(vp);
-    }
-  }
-}
-
-// The running state of a warp's 8 query heads over its keys.
+// The running state of a warp's 8 query heads over its keys. With k = kPBits - ve, probabilities are kept
+// as 2^(score - m + k), so that times a V scale (at most 2^(ve + 2)) they fit f16.
 template <int D, int NG>
 struct Acc {
-  float o[D / 16][4];       // O^T tiles of the codes: (channel gid | gid + 8 of the tile, heads 2 tig, 2 tig + 1)
-  float m[2], l[2];         // of heads 2 tig and 2 tig + 1; l and zs: this lane's keys alone
-  float zs[2][NG];          // sum P * zero
-  int ve;                   // V scales enter f16 times vf = 2^(kPBits - ve)
-  float vf, vlim;           // and are at most vlim
+  float o[D / 16][4];  // O^T tiles of the codes: (channel gid | gid + 8 of the tile, heads 2 tig, 2 tig + 1)
+  float m[2], l[2];    // of heads 2 tig and 2 tig + 1; l and zs: this lane's keys alone
+  float zs[2][NG];     // sum P * zero
+  float k, vlim;       // the exponent above, and the scales it holds for
 };
 
-// One run of 16 keys; kTail: only the first `valid` of them count, and whatever the other slots hold (NaN
-// too) is taken out of the products.
-template <int D, int NG, bool kTail>
-ES_DEVICE void attend(Acc<D, NG>& A, const Run<D, NG>& r, const uint32_t (*qb)[4], const float* xs, const float (*sq)[NG],
-                      int gid, int valid) {
+// What a warp keeps of its query rows.
+template <int D, int NG>
+struct Query {
+  uint32_t b[D / 32][4];  // B fragments of S^T: head gid, the channels of this lane's K words
+  uint32_t zero;          // B fragment of the zeros' part: part tig of scale * sum q, by group
+  float xs[2];            // the scores' factor, of heads 2 tig and 2 tig + 1
+};
+
+// Two runs of 16 keys, at rec0 and rec1 (records, or a record and its second half of rows): two, so that
+// their dependent steps overlap. kTail: only the first `valid` of the 32 keys count, and whatever the other
+// slots hold (NaN too) is taken out of the products.
+template <int D, int NG, int BS, bool kTail>
+ES_DEVICE void attend(Acc<D, NG>& A, const Query<D, NG>& Q, bool first, const uint8_t* rec0, const uint8_t* rec1,
+                      int sub1, int gid, int tig, int valid) {
+  using R = Rec<D, NG, BS>;
   constexpr int KW = D / 32, VW = D / 64, MT = D / 16;
+  const int kr = key_of_row(gid);
   // S^T = K . q^T on the codes
-  float acc[NG][4];
+  uint32_t kw[2][2][KW];  // [run][row gid | gid + 8][word]
+  uint32_t kp[2][2][NG], vp[2][2][NG];
 #pragma unroll
-  for (int g = 0; g < NG; g++) acc[g][0] = acc[g][1] = acc[g][2] = acc[g][3] = 0.f;
+  for (int u = 0; u < 2; u++) {
 #pragma unroll
-  for (int w = 0; w < KW; w++) {
-    float* d = acc[NG == 2 ? (w & 1) : 0];
-    uint32_t wa = r.k[0][w], wb = r.k[1][w];
-    const uint32_t a0[4] = {wa & 0x000F000Fu, wb & 0x000F000Fu, wa & 0x00F000F0u, wb & 0x00F000F0u};
-    mma_f16_16816(d, a0, qb[w][0], qb[w][1]);
-    wa >>= 8, wb >>= 8;
-    const uint32_t a1[4] = {wa & 0x000F000Fu, wb & 0x000F000Fu, wa & 0x00F000F0u, wb & 0x00F000F0u};
-    mma_f16_16816(d, a1, qb[w][2], qb[w][3]);
-  }
-  // scores in the log2 domain: x[row i][head j]
-  float x[2][2], sv[2][NG], zv[2][NG];
-#pragma unroll
-  for (int i = 0; i < 2; i++) {
-    const bool in = !kTail || key_of_row(gid) + 8 * i < valid;
-    float t0 = 0.f, t1 = 0.f, u0 = 0.f, u1 = 0.f;
-#pragma unroll
-    for (int g = 0; g < NG; g++) {
-      const float s = pair_scale(r.kp[i][g]), z = pair_zero(r.kp[i][g]);
-      t0 = fmaf(s, acc[g][2 * i], t0);
-      t1 = fmaf(s, acc[g][2 * i + 1], t1);
-      u0 = fmaf(z, sq[0][g], u0);
-      u1 = fmaf(z, sq[1][g], u1);
-      sv[i][g] = in ? pair_scale(r.vp[i][g]) : 0.f;
-      zv[i][g] = in ? pair_zero(r.vp[i][g]) : 0.f;
+    for (int i = 0; i < 2; i++) {
+      const int row = (u ? sub1 : 0) * 16 + 8 * i + kr;
+      const uint8_t* rec = u ? rec1 : rec0;
+      const uint8_t* at = rec + row * R::kRow + tig * (D / 8);
+      if (D == 128) {
+        const uint4 w = *reinterpret_cast<const uint4*>(at);
+        kw[u][i][0] = w.x, kw[u][i][1] = w.y, kw[u][i][KW - 2] = w.z, kw[u][i][KW - 1] = w.w;
+      } else {
+        const uint2 w = *reinterpret_cast<const uint2*>(at);
+        kw[u][i][0] = w.x, kw[u][i][1] = w.y;
+      }
+      const uint8_t* mp = rec + R::kKMeta + row * R::kMeta;
+      if (NG == 2) {
+        const uint2 a = *reinterpret_cast<const uint2*>(mp);
+        const uint2 b = *reinterpret_cast<const uint2*>(mp + BS * R::kMeta);
+        kp[u][i][0] = a.x, kp[u][i][NG - 1] = a.y, vp[u][i][0] = b.x, vp[u][i][NG - 1] = b.y;
+      } else {
+        kp[u][i][0] = *reinterpret_cast<const uint32_t*>(mp);
+        vp[u][i][0] = *reinterpret_cast<const uint32_t*>(mp + BS * R::kMeta);
+      }
     }
-    x[i][0] = in ? fmaf(t0, xs[0], u0) : -INFINITY;
-    x[i][1] = in ? fmaf(t1, xs[1], u1) : -INFINITY;
   }
-  float smax = fmaxf(sv[0][0], sv[1][0]);
-  if (NG == 2) smax = fmaxf(smax, fmaxf(sv[0][NG - 1], sv[1][NG - 1]));
-  const bool up = fmaxf(x[0][0], x[1][0]) > A.m[0] + kSlack || fmaxf(x[0][1], x[1][1]) > A.m[1] + kSlack || smax > A.vlim;
-  if (__any_sync(0xffffffffu, up)) {
-    float mt[2] = {fmaxf(x[0][0], x[1][0]), fmaxf(x[0][1], x[1][1])};
+  float acc[2][NG][4];
+#pragma unroll
+  for (int u = 0; u < 2; u++)
+#pragma unroll
+    for (int g = 0; g < NG; g++) acc[u][g][0] = acc[u][g][1] = acc[u][g][2] = acc[u][g][3] = 0.f;
+#pragma unroll
+  for (int w = 0; w < KW; w++)
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      float* d = acc[u][NG == 2 ? (w & 1) : 0];
+      uint32_t wa = kw[u][0][w], wb = kw[u][1][w];
+      const uint32_t a0[4] = {wa & 0x000F000Fu, wb & 0x000F000Fu, wa & 0x00F000F0u, wb & 0x00F000F0u};
+      mma_f16_16816(d, a0, Q.b[w][0], Q.b[w][1]);
+      wa >>= 8, wb >>= 8;
+      const uint32_t a1[4] = {wa & 0x000F000Fu, wb & 0x000F000Fu, wa & 0x00F000F0u, wb & 0x00F000F0u};
+      mma_f16_16816(d, a1, Q.b[w][2], Q.b[w][3]);
+    }
+  // x[run][row i][head j] = score - m + k in the log2 domain
+  float x[2][2][2];
+  float top[2] = {-INFINITY, -INFINITY}, smax = 0.f;
+#pragma unroll
+  for (int u = 0; u < 2; u++) {
+    float z[4];
+    // (one group: the scale in the low half meets a zero of B)
+    if (NG == 2)
+      mma_bf16_1688(z, __byte_perm(kp[u][0][0], kp[u][0][NG - 1], 0x7632), __byte_perm(kp[u][1][0], kp[u][1][NG - 1], 0x7632),
+                    Q.zero, A.k - A.m[0], A.k - A.m[1]);
+    else
+      mma_bf16_1688(z, kp[u][0][0], kp[u][1][0], Q.zero, A.k - A.m[0], A.k - A.m[1]);
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const bool in = !kTail || 16 * u + 8 * i + kr < valid;
+      float t0 = pair_scale(kp[u][i][0]) * acc[u][0][2 * i], t1 = pair_scale(kp[u][i][0]) * acc[u][0][2 * i + 1];
+      if (NG == 2) {
+        t0 = fmaf(pair_scale(kp[u][i][NG - 1]), acc[u][NG - 1][2 * i], t0);
+        t1 = fmaf(pair_scale(kp[u][i][NG - 1]), acc[u][NG - 1][2 * i + 1], t1);
+      }
+#pragma unroll
+      for (int g = 0; g < NG; g++) {
+        if (!in) vp[u][i][g] = 0;
+        smax = fmaxf(smax, pair_scale(vp[u][i][g]));
+      }
+      x[u][i][0] = in ? fmaf(t0, Q.xs[0], z[2 * i]) : -INFINITY;
+      x[u][i][1] = in ? fmaf(t1, Q.xs[1], z[2 * i + 1]) : -INFINITY;
+      top[0] = fmaxf(top[0], x[u][i][0]);
+      top[1] = fmaxf(top[1], x[u][i][1]);
+    }
+  }
+  if (__any_sync(0xffffffffu, first || fmaxf(top[0], top[1]) > A.k + kSlack || smax > A.vlim)) {
 #pragma unroll
     for (int s = 4; s < 32; s <<= 1) {
-      mt[0] = fmaxf(mt[0], __shfl_xor_sync(0xffffffffu, mt[0], s));
-      mt[1] = fmaxf(mt[1], __shfl_xor_sync(0xffffffffu, mt[1], s));
+      top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], s));
+      top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], s));
       smax = fmaxf(smax, __shfl_xor_sync(0xffffffffu, smax, s));
     }
-    float c[2];
-#pragma unroll
-    for (int j = 0; j < 2; j++) {
-      const float mn = fmaxf(A.m[j], mt[j]);
-      c[j] = A.m[j] == -INFINITY ? 0.f : ex2(A.m[j] - mn);
-      A.m[j] = mn;
-      A.l[j] *= c[j];
-#pragma unroll
-      for (int g = 0; g < NG; g++) A.zs[j][g] *= c[j];
-    }
+    float dk = 0.f;  // what k falls by
     if (smax > A.vlim) {
       const int e = exponent(smax) + 1;
-      const float f = pow2i(max(-126, A.ve - e));
-      c[0] *= f, c[1] *= f;
-      A.ve = e;
-      A.vf = pow2i((int)kPBits - e);
+      const float k = (float)(kPBits - e);
+      dk = A.k - k;
+      A.k = k;
       A.vlim = pow2i(e + 2);
     }
 #pragma unroll
-    for (int i = 0; i < MT; i++) A.o[i][0] *= c[0], A.o[i][1] *= c[1], A.o[i][2] *= c[0], A.o[i][3] *= c[1];
+    for (int j = 0; j < 2; j++) {
+      // the maximum: of the first keys as it is (none of them counted: left where it is), later the larger
+      const float up = top[j] - (A.k + dk);
+      const float dm = first ? (up == -INFINITY ? 0.f : up) : fmaxf(up, 0.f);
+      A.m[j] += dm;
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) x[u][i][j] -= dm + dk;
+      const float c = ex2(-(dm + dk));
+      if (!first) {
+        A.l[j] *= c;
+#pragma unroll
+        for (int g = 0; g < NG; g++) A.zs[j][g] *= c;
+#pragma unroll
+        for (int i = 0; i < MT; i++) A.o[i][j] *= c, A.o[i][2 + j] *= c;
+      }
+    }
   }
   // P, its sums, and P * scale as the B fragments of O^T (keys along k): transposed in registers
-  float pr[2][2];
+  uint32_t pb[2][NG][2];
 #pragma unroll
-  for (int i = 0; i < 2; i++)
-#pragma unroll
-    for (int j = 0; j < 2; j++) {
-      pr[i][j] = ex2(x[i][j] - A.m[j]);
-      A.l[j] += pr[i][j];
-#pragma unroll
-      for (int g = 0; g < NG; g++) A.zs[j][g] = fmaf(pr[i][j], zv[i][g], A.zs[j][g]);
-    }
-  uint32_t pb[NG][2];
-#pragma unroll
-  for (int g = 0; g < NG; g++)
+  for (int u = 0; u < 2; u++)
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-      const float s = sv[i][g] * A.vf;
-      pb[g][i] = transpose8(pack_f16x2(pr[i][0] * s, pr[i][1] * s));
+      const float p0 = ex2(x[u][i][0]), p1 = ex2(x[u][i][1]);
+      A.l[0] += p0;
+      A.l[1] += p1;
+#pragma unroll
+      for (int g = 0; g < NG; g++) {
+        const float z = pair_zero(vp[u][i][g]), s = pair_scale(vp[u][i][g]);
+        A.zs[0][g] = fmaf(p0, z, A.zs[0][g]);
+        A.zs[1][g] = fmaf(p1, z, A.zs[1][g]);
+        pb[u][g][i] = transpose8(pack_f16x2(p0 * s, p1 * s));
+      }
     }
   // O^T += V^T . P^T on the codes: rows gid and gid + 8 of tile (w, j) are channels 2 j and 2 j + 1 of
-  // word w, a register's halves the keys of rows 2 tig and 2 tig + 1
+  // word w, a register's halves the keys of rows 2 tig and 2 tig + 1. Even j keep their byte whole, c_j +
+  // 16 c_{j + 1}, and odd j take 16 c_{j + 1} out of it (subtracted in the end): a mask less a register.
 #pragma unroll
-  for (int w = 0; w < VW; w++) {
-    const int g = NG == 2 ? w : 0;
-    uint32_t e0 = __byte_perm(r.v[0][w], r.v[1][w], 0x5410), d0 = __byte_perm(r.v[0][w], r.v[1][w], 0x7632);
-    uint32_t e1 = __byte_perm(r.v[2][w], r.v[3][w], 0x5410), d1 = __byte_perm(r.v[2][w], r.v[3][w], 0x7632);
+  for (int u = 0; u < 2; u++) {
+    uint32_t v[4][VW];
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const uint32_t a0[4] = {e0 & 0x000F000Fu, d0 & 0x000F000Fu, e1 & 0x000F000Fu, d1 & 0x000F000Fu};
-      mma_f16_16816(A.o[w * 4 + 2 * h], a0, pb[g][0], pb[g][1]);
-      const uint32_t a1[4] = {e0 & 0x00F000F0u, d0 & 0x00F000F0u, e1 & 0x00F000F0u, d1 & 0x00F000F0u};
-      mma_f16_16816(A.o[w * 4 + 2 * h + 1], a1, pb[g][0], pb[g][1]);
-      e0 >>= 8, d0 >>= 8, e1 >>= 8, d1 >>= 8;
+    for (int j = 0; j < 4; j++) {
+      const int row = (u ? sub1 : 0) * 16 + 8 * (j >> 1) + ((j & 1) ? (tig ^ 1) + 4 : tig);
+      const uint8_t* at = (u ? rec1 : rec0) + R::kV + row * R::kRow + gid * (D / 16);
+      if (D == 128) {
+        const uint2 w = *reinterpret_cast<const uint2*>(at);
+        v[j][0] = w.x, v[j][VW - 1] = w.y;
+      } else {
+        v[j][0] = *reinterpret_cast<const uint32_t*>(at);
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < VW; w++) {
+      const int g = NG == 2 ? w : 0;
+      const uint32_t r[4] = {__byte_perm(v[0][w], v[1][w], 0x5410), __byte_perm(v[0][w], v[1][w], 0x7632),
+                             __byte_perm(v[2][w], v[3][w], 0x5410), __byte_perm(v[2][w], v[3][w], 0x7632)};
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        uint32_t a0[4], a1[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          a0[e] = h ? __byte_perm(r[e], 0u, 0x4341) : r[e] & 0x00FF00FFu;
+          a1[e] = a0[e] & 0x00F000F0u;
+        }
+        mma_f16_16816(A.o[w * 4 + 2 * h], a0, pb[u][g][0], pb[u][g][1]);
+        mma_f16_16816(A.o[w * 4 + 2 * h + 1], a1, pb[u][g][0], pb[u][g][1]);
+      }
     }
   }
 }
 
 template <int D, int NG, int BS>
-__global__ void __launch_bounds__(kDecThreads, 4) decode_kernel(DecodeParams p) {
+__global__ void __launch_bounds__(kDecThreads, kDecCtas) decode_kernel(DecodeParams p) {
   using R = Rec<D, NG, BS>;
   using C = Ring<D, NG, BS>;
   constexpr int KW = D / 32;  // K words a lane holds of a key
   constexpr int VW = D / 64;  // V words
-  constexpr int ST = C::kStages;
+  constexpr int PB = C::kStep, ST = C::kSteps;
   extern __shared__ __align__(128) uint8_t smem[];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -311,24 +351,26 @@ __global__ void __launch_bounds__(kDecThreads, 4) decode_kernel(DecodeParams p) 
   int ids = entries(0);
   const uint8_t* head_base = p.cache + (int64_t)kvh * R::kBytes;
   const uint64_t pol = ptx::policy_evict_first();
-  auto issue = [&](int i) {
-    const int64_t blk = __shfl_sync(0xffffffffu, ids, i & 31);
+  int issued = 0;  // blocks whose copies are on the way or done
+  auto issue = [&](int stage) {  // the next step's
+    if (issued != 0 && (issued & 31) == 0) ids = entries(issued);
+    const int n = min(PB, blocks - issued);
+    const int64_t b0 = __shfl_sync(0xffffffffu, ids, issued & 31), b1 = __shfl_sync(0xffffffffu, ids, (issued + PB - 1) & 31);
     if (lane == 0) {
-      ptx::mbar_arrive_expect_tx(&full[i % ST], R::kBytes);
-      ptx::bulk_g2s_hint(ring + i % ST * R::kBytes, head_base + blk * p.s_block, R::kBytes, &full[i % ST], pol);
+      ptx::mbar_arrive_expect_tx(&full[stage], n * R::kBytes);
+      uint8_t* dst = ring + stage * PB * R::kBytes;
+      ptx::bulk_g2s_hint(dst, head_base + b0 * p.s_block, R::kBytes, &full[stage], pol);
+      if (n == 2) ptx::bulk_g2s_hint(dst + R::kBytes, head_base + b1 * p.s_block, R::kBytes, &full[stage], pol);
     }
+    issued += n;
   };
-  int issued = min(ST, blocks);
-  for (int i = 0; i < issued; i++) issue(i);
+  for (int i = 0; i < ST && issued < blocks; i++) issue(i);
 
-  // the query: B fragments of S^T (head gid; k = the channels of this lane's K words), scaled to <= 2^10
-  uint32_t qb[KW][4];
-  float xs[2], sq[2][NG];  // of heads 2 tig and 2 tig + 1: the scores' factor, and scale * sum q by group
+  // the query, scaled to <= 2^10
+  Query<D, NG> Q;
   {
     float qv[KW][8];
-    float qmax = 0.f, sum[NG];
-#pragma unroll
-    for (int g = 0; g < NG; g++) sum[g] = 0.f;
+    float qmax = 0.f, sum[2] = {0.f, 0.f};
     const __nv_bfloat16* qr = p.q + (int64_t)b * p.q_stride + (int64_t)(head0 + min(gid, heads - 1)) * D;
 #pragma unroll
     for (int w = 0; w < KW; w++) {
@@ -339,31 +381,34 @@ __global__ void __launch_bounds__(kDecThreads, 4) decode_kernel(DecodeParams p) 
       for (int i = 0; i < 8; i++) {
         if (gid >= heads) qv[w][i] = 0.f;
         qmax = fmaxf(qmax, fabsf(qv[w][i]));
-        sum[NG == 2 ? (w & 1) : 0] += qv[w][i];
+        sum[NG == 2 ? (w & 1) : 1] += qv[w][i];
       }
     }
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
       qmax = fmaxf(qmax, __shfl_xor_sync(0xffffffffu, qmax, o));
 #pragma unroll
-      for (int g = 0; g < NG; g++) sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], o);
+      for (int g = 0; g < 2; g++) sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], o);
     }
     const int e = exponent(qmax);
     const float f = pow2i(9 - e), f16th = f * 0.0625f;
 #pragma unroll
     for (int w = 0; w < KW; w++) {
-      qb[w][0] = pack_f16x2(qv[w][0] * f, qv[w][1] * f);
-      qb[w][1] = pack_f16x2(qv[w][2] * f16th, qv[w][3] * f16th);
-      qb[w][2] = pack_f16x2(qv[w][4] * f, qv[w][5] * f);
-      qb[w][3] = pack_f16x2(qv[w][6] * f16th, qv[w][7] * f16th);
+      Q.b[w][0] = pack_f16x2(qv[w][0] * f, qv[w][1] * f);
+      Q.b[w][1] = pack_f16x2(qv[w][2] * f16th, qv[w][3] * f16th);
+      Q.b[w][2] = pack_f16x2(qv[w][4] * f, qv[w][5] * f);
+      Q.b[w][3] = pack_f16x2(qv[w][6] * f16th, qv[w][7] * f16th);
     }
     const float x = p.scale_log2 * pow2i(24 - 9 + e);
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-      xs[i] = __shfl_sync(0xffffffffu, x, (2 * tig + i) * 4);
+    for (int i = 0; i < 2; i++) Q.xs[i] = __shfl_sync(0xffffffffu, x, (2 * tig + i) * 4);
+    // scale * sum q in three terms of 8 bits, lane tig the tig-th: (first group, second), or with one group
+    // (0, the sum), which meets (scale, zero) of a key as stored
+    float t[2] = {p.scale_log2 * sum[0], p.scale_log2 * sum[1]};
 #pragma unroll
-      for (int g = 0; g < NG; g++) sq[i][g] = p.scale_log2 * __shfl_sync(0xffffffffu, sum[g], (2 * tig + i) * 4);
-    }
+    for (int i = 0; i < 2; i++)
+      if (i < tig) t[0] -= bf2f(f2bf(t[0])), t[1] -= bf2f(f2bf(t[1]));
+    Q.zero = tig < 3 ? ptx::pack_bf16x2(t[0], t[1]) : 0u;
   }
 
   Acc<D, NG> A;
@@ -371,38 +416,31 @@ __global__ void __launch_bounds__(kDecThreads, 4) decode_kernel(DecodeParams p) 
   for (int i = 0; i < D / 16; i++) A.o[i][0] = A.o[i][1] = A.o[i][2] = A.o[i][3] = 0.f;
 #pragma unroll
   for (int j = 0; j < 2; j++) {
-    A.m[j] = -INFINITY, A.l[j] = 0.f;
+    A.m[j] = 0.f, A.l[j] = 0.f;
 #pragma unroll
     for (int g = 0; g < NG; g++) A.zs[j][g] = 0.f;
   }
-  A.ve = -90;
-  A.vf = pow2i((int)kPBits + 90);
+  A.k = 0.f;
   A.vlim = 0.f;
 
-  for (int i = 0; i < blocks; i++) {
-    const uint8_t* rec = ring + i % ST * R::kBytes;
-    if (!__all_sync(0xffffffffu, ptx::mbar_wait(&full[i % ST], (i / ST) & 1))) {
+  int stage = 0, phase = 0;
+  for (int i = 0; i < blocks; i += PB) {
+    if (!__all_sync(0xffffffffu, ptx::mbar_wait(&full[stage], phase))) {
       // the copies on their way have to land before the warp leaves
-      for (int k = i; k < issued; k++) ptx::mbar_wait(&full[k % ST], (k / ST) & 1);
+      for (int k = i / PB; k * PB < issued; k++) ptx::mbar_wait(&full[k % ST], (k / ST) & 1);
       if (lane == 0 && p.status) atomicExch(p.status, (int)kTimeout);
       return;
     }
-#pragma unroll
-    for (int sub = 0; sub < BS / 16; sub++) {
-      const int valid = s1 - s0 - i * BS - sub * 16;
-      if (valid <= 0) break;
-      Run<D, NG> r;
-      load_run<D, NG, BS>(r, rec, sub, gid, tig);
-      if (sub == BS / 16 - 1 && issued < blocks) {
-        __syncwarp();  // every lane has read the stage
-        if ((issued & 31) == 0) ids = entries(issued);
-        issue(issued++);
-      }
-      if (valid >= 16)
-        attend<D, NG, false>(A, r, qb, xs, sq, gid, 16);
-      else
-        attend<D, NG, true>(A, r, qb, xs, sq, gid, valid);
-    }
+    const uint8_t* rec0 = ring + stage * PB * R::kBytes;
+    const uint8_t* rec1 = PB == 2 ? rec0 + R::kBytes : rec0;  // (of a block the split lacks: not counted)
+    const int valid = s1 - s0 - i * BS;
+    if (valid >= 32)
+      attend<D, NG, BS, false>(A, Q, i == 0, rec0, rec1, 2 - PB, gid, tig, 32);
+    else
+      attend<D, NG, BS, true>(A, Q, i == 0, rec0, rec1, 2 - PB, gid, tig, valid);
+    __syncwarp();  // every lane has read the step's stage
+    if (issued < blocks) issue(stage);
+    if (++stage == ST) stage = 0, phase ^= 1;
   }
 
   // the lanes' sums; the output with the codes' factor and the zeros' part
@@ -415,7 +453,6 @@ __global__ void __launch_bounds__(kDecThreads, 4) decode_kernel(DecodeParams p) 
       for (int g = 0; g < NG; g++) A.zs[j][g] += __shfl_xor_sync(0xffffffffu, A.zs[j][g], s);
     }
   }
-  const float of = pow2i(24 - (int)kPBits + A.ve);
 #pragma unroll
   for (int j = 0; j < 2; j++) {
     const int h = 2 * tig + j;
@@ -424,12 +461,15 @@ __global__ void __launch_bounds__(kDecThreads, 4) decode_kernel(DecodeParams p) 
 #pragma unroll
     for (int w = 0; w < VW; w++) {
       float y[8];  // channels 8 (gid + 8 w) and up
+      const float z = A.zs[j][NG == 2 ? w : 0];
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const float f = (i & 1) ? of * 0.0625f : of, z = A.zs[j][NG == 2 ? w : 0];
-        y[2 * i] = fmaf(A.o[w * 4 + i][j], f, z);
-        y[2 * i + 1] = fmaf(A.o[w * 4 + i][2 + j], f, z);
-      }
+      for (int i = 0; i < 4; i += 2)
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+          const float odd = A.o[w * 4 + i + 1][2 * c + j], even = A.o[w * 4 + i][2 * c + j] - odd;
+          y[2 * i + c] = fmaf(even, 16777216.f, z);         // 2^24: a code in bits 0..3
+          y[2 * i + 2 + c] = fmaf(odd, 1048576.f, z);       // 2^20: in bits 4..7
+        }
       const int ch = 8 * (gid + 8 * w);
       if (ns == 1) {
 #pragma unroll
@@ -442,7 +482,7 @@ __global__ void __launch_bounds__(kDecThreads, 4) decode_kernel(DecodeParams p) 
       }
     }
     if (ns > 1 && gid == 0)
-      *reinterpret_cast<float2*>(p.part_ml + ((row0 + h) * p.max_splits + split) * 2) = make_float2(A.m[j], A.l[j]);
+      *reinterpret_cast<float2*>(p.part_ml + ((row0 + h) * p.max_splits + split) * 2) = make_float2(A.m[j] - A.k, A.l[j]);
   }
 }
 
