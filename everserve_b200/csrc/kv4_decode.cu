@@ -40,11 +40,11 @@ constexpr float kSlack = 6.f;       // log2 of how far a score may pass the runn
 constexpr int kPBits = 7;           // P * scale enters f16 as at most 2^(6 + 2 + 7) = 2^15
 
 // Keys of a split: short where a lone sequence needs the warps, longer where the ends of a split (query
-// in, partial result out) would cost more than they bring. At most 32 blocks, whose table entries a warp
-// holds one a lane.
-__host__ __device__ __forceinline__ int part_of(int n) { return n <= 1024 ? 128 : n <= 4096 ? 256 : 512; }
+// in, partial result out) cost more than they bring (64 sequences of 1K keys: 29.5 us at 256, 32.2 at 128;
+// 48 of up to 8K: 57.0 at 512, 58.1 at 256).
+__host__ __device__ __forceinline__ int part_of(int n) { return n <= 1024 ? 256 : 512; }
 // Splits of a history of n keys.
-__host__ __device__ __forceinline__ int splits_of(int n) { return n <= 128 ? 1 : (n + part_of(n) - 1) / part_of(n); }
+__host__ __device__ __forceinline__ int splits_of(int n) { return n <= 256 ? 1 : (n + part_of(n) - 1) / part_of(n); }
 
 template <int D, int NG, int BS>
 struct Ring {
@@ -486,23 +486,67 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas) decode_kernel(DecodePar
   }
 }
 
-// out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i over a row's splits, in an order of its own: warp w
-// takes splits w, w + 8, ..., then the warps add in order. One CTA per (sequence, query head); the loads of
-// four splits are on the way at a time.
+// out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i over a row's splits. A row of at most kFew splits is one
+// warp's, in order; a longer one is a CTA's: warp w takes splits w, w + 8, ..., then the warps add in order.
+// (The rule is the row's own count, so its bits do not depend on the launch.) Four splits' loads are on the
+// way at a time.
 constexpr int kMergeWarps = 8;
+constexpr int kFew = 16;
+
 template <int D>
+struct Part {
+  static constexpr int E = D / 32;  // neighbouring channels of a lane
+  float acc[E], l;
+  // splits first, first + step, ... of a row whose maximum is mx
+  ES_DEVICE void sum(const float* po, const float2* ml, int ns, int first, int step, float mx, int lane) {
+    l = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; e++) acc[e] = 0.f;
+#pragma unroll 4
+    for (int i = first; i < ns; i += step) {
+      const float2 t = ml[i];
+      const float f = t.x == mx ? 1.f : ex2(t.x - mx);
+      l = fmaf(t.y, f, l);
+      float v[E];
+      if (E == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(po + (int64_t)i * D + E * lane);
+        v[0] = x.x, v[1] = x.y, v[E - 2] = x.z, v[E - 1] = x.w;
+      } else {
+        const float2 x = *reinterpret_cast<const float2*>(po + (int64_t)i * D + E * lane);
+        v[0] = x.x, v[1] = x.y;
+      }
+#pragma unroll
+      for (int e = 0; e < E; e++) acc[e] = fmaf(v[e], f, acc[e]);
+    }
+  }
+};
+
+// kRows: a CTA takes kMergeWarps rows, a warp each (no row has more than kFew splits); else one row.
+template <int D, bool kRows>
 __global__ void __launch_bounds__(kMergeWarps * 32)
     merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, const int* __restrict__ ctx_lens,
-                 __nv_bfloat16* __restrict__ out, int hq, int max_splits, int max_keys) {
-  constexpr int E = D / 32;  // neighbouring channels of a lane
-  __shared__ float so[kMergeWarps][D], sl[kMergeWarps], smx[kMergeWarps];
+                 __nv_bfloat16* __restrict__ out, int64_t rows, int hq, int max_splits, int max_keys) {
+  constexpr int E = D / 32;
+  __shared__ float so[kRows ? 1 : kMergeWarps][D], sl[kMergeWarps], smx[kMergeWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t row = kRows ? (int64_t)blockIdx.x * kMergeWarps + warp : blockIdx.x;
   pdl_wait();
   pdl_launch();
-  const int ns = min(max_splits, splits_of(min(ctx_lens[blockIdx.y], max_keys)));
+  if (row >= rows) return;
+  const int ns = min(max_splits, splits_of(min(ctx_lens[row / hq], max_keys)));
   if (ns <= 1) return;  // written by the split itself
-  const int64_t row = (int64_t)blockIdx.y * hq + blockIdx.x;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float2* ml = reinterpret_cast<const float2*>(part_ml) + row * max_splits;
+  const float* po = part_o + row * max_splits * D;
+  Part<D> a;
+  if (ns <= kFew) {
+    if (!kRows && warp > 0) return;
+    const float mx = warp_max(lane < ns ? ml[lane].x : -INFINITY);
+    a.sum(po, ml, ns, 0, 1, mx, lane);
+#pragma unroll
+    for (int e = 0; e < E; e++) out[row * D + E * lane + e] = f2bf(a.acc[e] / a.l);
+    return;
+  }
+  if (kRows) return;
   float mx = -INFINITY;
   for (int i = threadIdx.x; i < ns; i += kMergeWarps * 32) mx = fmaxf(mx, ml[i].x);
   mx = warp_max(mx);
@@ -511,29 +555,10 @@ __global__ void __launch_bounds__(kMergeWarps * 32)
   mx = smx[0];
 #pragma unroll
   for (int w = 1; w < kMergeWarps; w++) mx = fmaxf(mx, smx[w]);
-  float acc[E], l = 0.f;
+  a.sum(po, ml, ns, warp, kMergeWarps, mx, lane);
 #pragma unroll
-  for (int e = 0; e < E; e++) acc[e] = 0.f;
-  const float* po = part_o + row * max_splits * D + E * lane;
-#pragma unroll 4
-  for (int i = warp; i < ns; i += kMergeWarps) {
-    const float2 t = ml[i];
-    const float f = t.x == mx ? 1.f : ex2(t.x - mx);
-    l = fmaf(t.y, f, l);
-    float v[E];
-    if (E == 4) {
-      const float4 x = *reinterpret_cast<const float4*>(po + (int64_t)i * D);
-      v[0] = x.x, v[1] = x.y, v[E - 2] = x.z, v[E - 1] = x.w;
-    } else {
-      const float2 x = *reinterpret_cast<const float2*>(po + (int64_t)i * D);
-      v[0] = x.x, v[1] = x.y;
-    }
-#pragma unroll
-    for (int e = 0; e < E; e++) acc[e] = fmaf(v[e], f, acc[e]);
-  }
-#pragma unroll
-  for (int e = 0; e < E; e++) so[warp][E * lane + e] = acc[e];
-  if (lane == 0) sl[warp] = l;
+  for (int e = 0; e < E; e++) so[warp][E * lane + e] = a.acc[e];
+  if (lane == 0) sl[warp] = a.l;
   __syncthreads();
   if (threadIdx.x < D) {
     const int c = threadIdx.x;
@@ -555,8 +580,13 @@ cudaError_t launch_decode(const DecodeParams& p, int B, cudaStream_t stream) {
   e = launch_ex(decode_kernel<D, NG, BS>, dim3((p.max_splits + kDecWarps - 1) / kDecWarps, p.hkv * p.head_tiles, B),
                 dim3(kDecThreads), C::kSmem, stream, 0, p);
   if (e != cudaSuccess || p.max_splits == 1) return e;
-  return launch_ex(merge_kernel<D>, dim3(p.hq, B), dim3(kMergeWarps * 32), 0, stream, 0, (const float*)p.part_o,
-                   (const float*)p.part_ml, p.ctx_lens, p.out, p.hq, p.max_splits, p.bt_cols * BS);
+  const int64_t rows = (int64_t)B * p.hq;
+  auto merge = [&](auto kernel, int64_t grid) {
+    return launch_ex(kernel, dim3((unsigned)grid), dim3(kMergeWarps * 32), 0, stream, 0, (const float*)p.part_o,
+                     (const float*)p.part_ml, p.ctx_lens, p.out, rows, p.hq, p.max_splits, p.bt_cols * BS);
+  };
+  return p.max_splits <= kFew ? merge(merge_kernel<D, true>, (rows + kMergeWarps - 1) / kMergeWarps)
+                              : merge(merge_kernel<D, false>, rows);
 }
 
 }  // namespace kv4
@@ -565,8 +595,7 @@ int64_t kv4_max_splits(int64_t max_len) {
   // the most of any length up to max_len: the count falls where the splits get longer
   const int n = (int)std::min<int64_t>(max_len, INT32_MAX - 1024);
   int most = kv4::splits_of(n);
-  for (const int top : {1024, 4096})
-    if (n > top) most = std::max(most, kv4::splits_of(top));
+  if (n > 1024) most = std::max(most, kv4::splits_of(1024));
   return most;
 }
 
@@ -593,7 +622,7 @@ cudaError_t launch_kv4_decode(const Kv4DecodeArgs& a, cudaStream_t stream) {
   p.head_tiles = (a.hq / a.c.hkv + 7) / 8;
   p.max_splits = a.max_splits;
   p.scale_log2 = a.scale * kv4::kLog2eF;
-  if ((int64_t)p.hkv * p.head_tiles > 65535 || p.hq > 65535) return cudaErrorInvalidValue;
+  if ((int64_t)p.hkv * p.head_tiles > 65535 || (int64_t)a.B * a.hq > INT32_MAX) return cudaErrorInvalidValue;
   return kv4::pick(a.c.d, a.c.groups, a.c.block_size, [&](auto d, auto ng, auto bs) {
     return kv4::launch_decode<d, ng, bs>(p, a.B, stream);
   });
