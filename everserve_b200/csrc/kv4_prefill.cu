@@ -1,18 +1,24 @@
 // Causal attention of a step's new rows over their sequences' paged history held in 4 bits (tcgen05, TMEM).
 //
 // The products are large here (128 and more query rows share a key), so a key's codes are turned into
-// bf16 values once for 256 query rows and the tensor cores do the rest: v = scale * c + zero, c exact in
-// bf16 and the multiply-add rounded once. The query rows of one kv head's whole group are packed into the
+// f16 values once for 256 query rows and the tensor cores do the rest: v = scale * c + zero, c exact in
+// f16 and the multiply-add rounded once. The query rows of one kv head's whole group are packed into the
 // rows of a tile (row = token * G + head of the group), so grouped heads share the conversion too.
+//
+// f16 carries 11 bits where bf16 carries 8 (a key in bf16 alone would double the error of the output), but
+// fewer exponents. So each operand stands under a power of two of its own: a query row's, which its scores'
+// factor takes back; a key tile's of K, likewise; and a key tile's of V, which enters the exponent of that
+// tile's probabilities against the largest so far. None of them costs an operation per element.
 //
 // A CTA keeps to its SM and walks work items: 256 rows (two tiles of 128) of one sequence and kv head,
 // over a run of 128-key tiles. Its warps:
 //   * 8-11 turn tile j's codes (loaded a tile ahead, straight to registers) into K and V stages in shared
 //     memory, 128-byte swizzled;
 //   * 12 issues the MMAs: S_t = Q_t . K_j^T and O_t += P_t . V_j for t = 0, 1 in turn, P read from TMEM;
-//   * 0-3 and 4-7 do the softmax of tiles 0 and 1, a thread a row: S from TMEM, P back over it in bf16.
+//   * 0-3 and 4-7 do the softmax of tiles 0 and 1, a thread a row: S from TMEM, P back over it in f16.
 // While one tile's softmax runs, the tensor core works for the other. The running maximum moves (and O in
-// TMEM is rescaled) only when a score passes it by 2^8, so most tiles leave O alone. A row's sums are fp32.
+// TMEM is rescaled) only when a score passes it by 2^6, so most tiles leave O alone. A row's sums are fp32.
+// Registers go where they are needed: 184 a softmax thread (a row's 128 scores at once), 104 a converting one.
 //
 // A sequence with few rows and a long history is cut along its keys as well, into items whose results
 // (O, m, l) a second kernel joins. The cut depends on the sequence's own rows and keys and on the model's
@@ -33,7 +39,10 @@ constexpr int kRows = 128;  // rows of a tile (MMA M)
 constexpr int kKeys = 128;  // keys of a tile (MMA N of S, K of P.V)
 constexpr int kSoftThreads = 256;
 constexpr int kConvThreads = 128;
-constexpr int kPreThreads = kSoftThreads + kConvThreads + 32;
+constexpr int kPreThreads = kSoftThreads + kConvThreads + 128;  // (the MMA warp's group has three idle warps)
+constexpr int kSoftRegs = 184, kConvRegs = 104, kMmaRegs = 40;
+static_assert(kSoftRegs * kSoftThreads + kConvRegs * kConvThreads + kMmaRegs * 128 <= 128 * kPreThreads,
+              "the split draws on the registers of the launch, 128 a thread");
 constexpr int kTmem = 512;  // S0, S1 (128 columns each, P over them), O0, O1
 
 template <int D>
@@ -42,6 +51,15 @@ struct PreCfg {
   static constexpr int kTile = (D / 64) * kChunk;      // a bf16 tile of 128 rows
   static constexpr int kSmem = 1024 + 2 * kTile + 2 * 2 * kTile + 256;
 };
+
+constexpr float kPreSlack = 6.f;  // log2 of how far a score may pass the running maximum
+constexpr float kPreBits = 9.f;   // P enters f16 as at most 2^(6 + 9)
+constexpr int kTop = 13;          // operands are scaled to below 2^(kTop + 1)
+
+template <int N>
+ES_DEVICE void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+ES_DEVICE void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 struct PreParams {
   const __nv_bfloat16* q;  // [T, hq, D] rows of q_stride
@@ -130,19 +148,26 @@ ES_DEVICE void span(const PreParams& p, const Item& it, int& j0, int& j1, int& n
   if (it.split >= ns) j1 = j0;
 }
 
-// 8 codes -> 8 bf16 values
-ES_DEVICE uint4 values8(uint32_t w, __nv_bfloat162 s, __nv_bfloat162 z) {
-  const __nv_bfloat162 bias = __floats2bfloat162_rn(128.f, 128.f);
+// 8 codes -> 8 f16 values: a masked nibble under the exponent of 1024 (bits 0..3) or 64 (bits 4..7) is
+// 1024 + c or 64 + c
+ES_DEVICE uint4 values8(uint32_t w, __half2 s, __half2 z) {
   uint32_t r[4];
 #pragma unroll
-  for (int j = 0; j < 4; j++) {
-    const uint32_t h = ((w >> (4 * j)) & 0x000F000Fu) | 0x43004300u;  // 128 + c
-    const __nv_bfloat162 c = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&h), bias);
-    const __nv_bfloat162 v = __hfma2(c, s, z);
-    r[j] = *reinterpret_cast<const uint32_t*>(&v);
+  for (int h = 0; h < 2; h++) {
+    const uint32_t lo = (w & 0x000F000Fu) | 0x64006400u, hi = (w & 0x00F000F0u) | 0x54005400u;
+    const __half2 a = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&lo), __float2half2_rn(1024.f)), s, z);
+    const __half2 b = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&hi), __float2half2_rn(64.f)), s, z);
+    r[2 * h] = *reinterpret_cast<const uint32_t*>(&a);
+    r[2 * h + 1] = *reinterpret_cast<const uint32_t*>(&b);
+    w >>= 8;
   }
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
+
+// 2^e as a float, e in [-126, 127], and the exponent of a positive number (of its bits), clamped so that the
+// product of a query row's and a key tile's factor stays a normal number
+ES_DEVICE float pre_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+ES_DEVICE int pre_exponent(uint32_t bits) { return min(100, max(-40, (int)(bits >> 23) - 127)); }
 
 // What a converting thread holds of a key tile: 16-byte pieces (32 codes) of K and of V rows.
 template <int D, int NG>
@@ -152,45 +177,47 @@ struct Raw {
   uint32_t km[kPer][NG], vm[kPer][NG];
 };
 
+// The i-th piece of key tile j.
 template <int D, int NG, int BS>
-ES_DEVICE void load_raw(Raw<D, NG>& r, const PreParams& p, const Item& it, int j, int tid) {
+ES_DEVICE void load_raw(Raw<D, NG>& r, int i, const PreParams& p, const Item& it, int j, int tid) {
   using R = Rec<D, NG, BS>;
   constexpr int P = D / 32;
-  const int* bt = p.block_tables + (int64_t)it.seq * p.bt_stride;
+  const int key = j * kKeys + i * (kConvThreads / P) + tid / P;
+  r.k[i] = r.v[i] = make_uint4(0, 0, 0, 0);  // past the history: values of zero, whatever the slot holds
 #pragma unroll
-  for (int i = 0; i < P; i++) {
-    const int key = j * kKeys + i * (kConvThreads / P) + tid / P;
-    r.k[i] = r.v[i] = make_uint4(0, 0, 0, 0);  // past the history: values of zero, whatever the slot holds
-#pragma unroll
-    for (int g = 0; g < NG; g++) r.km[i][g] = r.vm[i][g] = 0;
-    if (key < it.ctx) {
-      int64_t blk = bt[key / BS];
-      if (blk < 0 || blk >= p.num_blocks) {  // not a block of this cache: reported, block 0 read instead
-        if (p.status) atomicExch(p.status, (int)kBadShape);
-        blk = 0;
-      }
-      const uint8_t* rec = p.cache + blk * p.s_block + (int64_t)it.head * R::kBytes;
-      const int off = key % BS;
-      r.k[i] = *reinterpret_cast<const uint4*>(rec + off * R::kRow + 16 * (tid % P));
-      r.v[i] = *reinterpret_cast<const uint4*>(rec + R::kV + off * R::kRow + 16 * (tid % P));
-      const uint32_t* km = reinterpret_cast<const uint32_t*>(rec + R::kKMeta + off * R::kMeta);
-      const uint32_t* vm = reinterpret_cast<const uint32_t*>(rec + R::kVMeta + off * R::kMeta);
-#pragma unroll
-      for (int g = 0; g < NG; g++) r.km[i][g] = km[g], r.vm[i][g] = vm[g];
+  for (int g = 0; g < NG; g++) r.km[i][g] = r.vm[i][g] = 0;
+  if (key < it.ctx) {
+    int64_t blk = p.block_tables[(int64_t)it.seq * p.bt_stride + key / BS];
+    if (blk < 0 || blk >= p.num_blocks) {  // not a block of this cache: reported, block 0 read instead
+      if (p.status) atomicExch(p.status, (int)kBadShape);
+      blk = 0;
     }
+    const uint8_t* rec = p.cache + blk * p.s_block + (int64_t)it.head * R::kBytes;
+    const int off = key % BS;
+    r.k[i] = *reinterpret_cast<const uint4*>(rec + off * R::kRow + 16 * (tid % P));
+    r.v[i] = *reinterpret_cast<const uint4*>(rec + R::kV + off * R::kRow + 16 * (tid % P));
+    const uint32_t* km = reinterpret_cast<const uint32_t*>(rec + R::kKMeta + off * R::kMeta);
+    const uint32_t* vm = reinterpret_cast<const uint32_t*>(rec + R::kVMeta + off * R::kMeta);
+#pragma unroll
+    for (int g = 0; g < NG; g++) r.km[i][g] = km[g], r.vm[i][g] = vm[g];
   }
 }
 
-// One piece of row `row` into a tile's swizzled layout.
+// The bits of a bound on a group's magnitudes.
+ES_DEVICE uint32_t bound_of(uint32_t pair) {
+  const float z = pair_zero(pair);
+  return __float_as_uint(fmaxf(fabsf(z), fabsf(fmaf(15.f, pair_scale(pair), z))));
+}
+
+// One piece of row `row` into a tile's swizzled layout, times f.
 template <int D, int NG>
-ES_DEVICE void store_piece(uint8_t* tile, int row, int piece, const uint4& codes, const uint32_t* meta) {
+ES_DEVICE void store_piece(uint8_t* tile, int row, int piece, const uint4& codes, const uint32_t* meta, float f) {
   const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
-  __nv_bfloat162 s[NG], z[NG];
+  __half2 s[NG], z[NG];
 #pragma unroll
   for (int g = 0; g < NG; g++) {
-    const uint32_t sp = __byte_perm(meta[g], meta[g], 0x1010), zp = __byte_perm(meta[g], meta[g], 0x3232);
-    s[g] = *reinterpret_cast<const __nv_bfloat162*>(&sp);
-    z[g] = *reinterpret_cast<const __nv_bfloat162*>(&zp);
+    s[g] = __float2half2_rn(pair_scale(meta[g]) * f);
+    z[g] = __float2half2_rn(pair_zero(meta[g]) * f);
   }
 #pragma unroll
   for (int i = 0; i < 4; i++) {
@@ -214,6 +241,9 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
   uint64_t* mma_done = bar + 12;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 13);
   __shared__ int s_fail;
+  __shared__ uint32_t s_bound[2][2][4];  // [tile parity][K, V][converting warp]: largest magnitudes' bits
+  __shared__ int s_exp[2][2];            // [stage][K, V]: the tile's exponents
+  __shared__ int s_qexp[2][kRows];       // [tile][row]: the query rows' exponents
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -242,36 +272,58 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
   bool ok = true;
   if (warp >= 8 && warp < 12) {
     // ---- codes to values ------------------------------------------------------------------------
+    regs_down<kConvRegs>();
     constexpr int P = D / 32;
     const int tid = threadIdx.x - kSoftThreads;
     uint32_t n = 0;  // key tiles converted so far, over all items
     for (int idx = blockIdx.x; ok && find_item(p, BS, idx, it); idx += gridDim.x) {
       span(p, it, j0, j1, ns);
       if (j0 >= j1) continue;
-      Raw<D, NG> nxt;
-      load_raw<D, NG, BS>(nxt, p, it, j0, tid);
+      Raw<D, NG> r;
+      int vr = -100;  // the largest of V's exponents so far
+#pragma unroll
+      for (int i = 0; i < P; i++) load_raw<D, NG, BS>(r, i, p, it, j0, tid);
       for (int j = j0; j < j1; j++, n++) {
-        const Raw<D, NG> r = nxt;
-        if (j + 1 < j1) load_raw<D, NG, BS>(nxt, p, it, j + 1, tid);
         const int s = n & 1;
+        uint32_t kb = 0, vb = 0;
+#pragma unroll
+        for (int i = 0; i < P; i++)
+#pragma unroll
+          for (int g = 0; g < NG; g++) kb = max(kb, bound_of(r.km[i][g])), vb = max(vb, bound_of(r.vm[i][g]));
+        kb = __reduce_max_sync(0xffffffffu, kb);
+        vb = __reduce_max_sync(0xffffffffu, vb);
+        if (lane == 0) s_bound[s][0][warp - 8] = kb, s_bound[s][1][warp - 8] = vb;
         if (n >= 2) ok = __all_sync(0xffffffffu, ptx::mbar_wait(&kv_empty[s], ((n >> 1) - 1) & 1));
-        if (!ok) break;
+        if (ptx::named_bar_or(1, kConvThreads, !ok)) {  // the converting warps leave together
+          ok = false;
+          break;
+        }
+        const uint32_t *bk = s_bound[s][0], *bv = s_bound[s][1];
+        const int ke = pre_exponent(max(max(bk[0], bk[1]), max(bk[2], bk[3])));
+        // (not far below the largest: a tile of small values leaves its probabilities' range alone)
+        const int ve = max(pre_exponent(max(max(bv[0], bv[1]), max(bv[2], bv[3]))), vr - 20);
+        vr = max(vr, ve);
+        if (tid == 0) s_exp[s][0] = ke, s_exp[s][1] = ve;
+        const float kf = pre_pow2(kTop - ke), vf = pre_pow2(kTop - ve);
         uint8_t* kt = kv_s + s * 2 * C::kTile;
 #pragma unroll
         for (int i = 0; i < P; i++) {
           const int row = i * (kConvThreads / P) + tid / P;
-          store_piece<D, NG>(kt, row, tid % P, r.k[i], r.km[i]);
-          store_piece<D, NG>(kt + C::kTile, row, tid % P, r.v[i], r.vm[i]);
+          store_piece<D, NG>(kt, row, tid % P, r.k[i], r.km[i], kf);
+          store_piece<D, NG>(kt + C::kTile, row, tid % P, r.v[i], r.vm[i], vf);
+          if (j + 1 < j1) load_raw<D, NG, BS>(r, i, p, it, j + 1, tid);
         }
         ptx::fence_proxy_async();
         ptx::mbar_arrive(&kv_full[s]);
       }
     }
     if (!ok) s_fail = 1;
-  } else if (warp == 12) {
-    // ---- MMA issuer -----------------------------------------------------------------------------
-    constexpr uint32_t idesc_s = ptx::idesc_bf16_f32(kRows, kKeys);
-    constexpr uint32_t idesc_o = ptx::idesc_bf16_f32_bmn(kRows, D);
+  } else if (warp >= 12) {
+    // ---- MMA issuer (the group's other warps idle) -------------------------------------------------
+    regs_down<kMmaRegs>();
+    ok = warp == 12;
+    constexpr uint32_t idesc_s = ptx::idesc_f16_f32(kRows, kKeys);
+    constexpr uint32_t idesc_o = ptx::idesc_f16_f32(kRows, D) | (1u << 16);  // V: MN-major
     uint32_t n = 0, items = 0;
     auto qk = [&](int t, int s) {  // S_t = Q_t . K^T
 #pragma unroll
@@ -320,19 +372,19 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
       }
       ok = __shfl_sync(0xffffffffu, (int)ok, 0);
     }
-    if (lane == 0) {
+    if (warp == 12 && lane == 0) {
       if (!ok) s_fail = 1;
       ptx::mma_commit(mma_done);  // nothing of this CTA is in flight past here
       ptx::mbar_wait(mma_done, 0);
     }
   } else {
     // ---- softmax --------------------------------------------------------------------------------
+    regs_up<kSoftRegs>();
     const int t = warp >> 2;
     const int r = threadIdx.x & 127;  // row of the tile (TMEM lane)
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_t = tmem + t * 128 + lane_base, o_t = tmem + 256 + t * 128 + lane_base;
     const int token = r / p.G, head = r - token * p.G;
-    const float c = p.scale_log2, slack = 8.f / c;
     uint32_t n = 0, items = 0;
     for (int idx = blockIdx.x; ok && find_item(p, BS, idx, it); idx += gridDim.x) {
       span(p, it, j0, j1, ns);
@@ -348,84 +400,112 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
           for (int i = 0; i < D / 8; i++) reinterpret_cast<uint4*>(out)[i] = make_uint4(0, 0, 0, 0);
         continue;
       }
-      // the tile's query rows: 16-byte units in memory's order, swizzled (a row past the sequence: zeros)
-      for (int u = threadIdx.x & 127; u < 128 * (D / 8); u += 128) {
+      // the tile's query rows, scaled row by row: D / 8 lanes a row, 16-byte units in memory's order, swizzled
+      // (a row past the sequence: zeros)
+      for (int u = r; u < kRows * (D / 8); u += 128) {
         const int rr = u / (D / 8), k = u % (D / 8);
         const int tk = rr / p.G, hh = rr - tk * p.G;
         uint4 v = make_uint4(0, 0, 0, 0);
         if (tk < p.tt && tok0 + tk < it.rows)
           v = *reinterpret_cast<const uint4*>(p.q + (int64_t)(it.row0 + tok0 + tk) * p.q_stride +
                                               (int64_t)(it.head * p.G + hh) * D + 8 * k);
-        *reinterpret_cast<uint4*>(q_s + t * C::kTile + (k >> 3) * C::kChunk + rr * 128 + (((k & 7) ^ (rr & 7)) << 4)) = v;
+        float f[8];
+        unpack8(v, f);
+        float mx = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(f[i]));
+#pragma unroll
+        for (int o = 1; o < D / 8; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const int e = pre_exponent(__float_as_uint(mx));
+        const float w = pre_pow2(kTop - e);
+        uint32_t h[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const __half2 x = __floats2half2_rn(f[2 * i] * w, f[2 * i + 1] * w);
+          h[i] = *reinterpret_cast<const uint32_t*>(&x);
+        }
+        *reinterpret_cast<uint4*>(q_s + t * C::kTile + (k >> 3) * C::kChunk + rr * 128 + (((k & 7) ^ (rr & 7)) << 4)) =
+            make_uint4(h[0], h[1], h[2], h[3]);
+        if (k == 0) s_qexp[t][rr] = e;
       }
       ptx::fence_proxy_async();
       ptx::mbar_arrive(&q_full[t]);
+      ptx::named_bar(2 + t, 128);
+      const float cq = p.scale_log2 * pre_pow2(s_qexp[t][r] - kTop);
 
+      // the running maximum in the log2 domain, the sum, and the exponent that O's values of V stand under
       float m = -INFINITY, l = 0.f;
+      int vrun = -100;
       for (int j = j0; j < j1; j++, n++) {
         ok = __all_sync(0xffffffffu, ptx::mbar_wait(&s_full[t], n & 1));
         if (!ok) break;
         ptx::tc_fence_after();
+        const float c = cq * pre_pow2(s_exp[n & 1][0] - kTop);
+        const int ve = s_exp[n & 1][1];
+        uint32_t v[128];
+#pragma unroll
+        for (int q = 0; q < 4; q++) ptx::tmem_ld32(s_t + q * 32, v + q * 32);
+        ptx::tmem_wait_ld();
         const int key0 = j * kKeys;
-        const bool masked = __any_sync(0xffffffffu, key0 + kKeys - 1 > pos);
-        float mx = -INFINITY;
-        uint32_t v[32];
+        if (__any_sync(0xffffffffu, key0 + kKeys - 1 > pos)) {
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-          ptx::tmem_ld32(s_t + q * 32, v);
-          ptx::tmem_wait_ld();
-          if (masked) {
-#pragma unroll
-            for (int i = 0; i < 32; i++)
-              if (key0 + q * 32 + i <= pos) mx = fmaxf(mx, __uint_as_float(v[i]));
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; i++) mx = fmaxf(mx, __uint_as_float(v[i]));
-          }
+          for (int i = 0; i < 128; i++)
+            if (key0 + i > pos) v[i] = 0xFF800000u;  // -infinity
         }
-        if (__any_sync(0xffffffffu, mx > m + slack)) {
-          const float mn = fmaxf(m, mx);
-          const float a = m == -INFINITY ? 0.f : ex2((m - mn) * c);
+        float mx[4];
+#pragma unroll
+        for (int q = 0; q < 4; q++) mx[q] = __uint_as_float(v[q]);
+#pragma unroll
+        for (int i = 4; i < 128; i++) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(v[i]));
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
+        if (__any_sync(0xffffffffu, top > m + kPreSlack || ve > vrun)) {
+          const float mn = fmaxf(m, top);
+          const float a = m == -INFINITY ? 0.f : ex2(m - mn);
+          const int vn = max(vrun, ve);
           m = mn;
           l *= a;
           if (j > j0) {
+            const float f = a * pre_pow2(max(-126, vrun - vn));
 #pragma unroll
             for (int q = 0; q < D / 32; q++) {
-              ptx::tmem_ld32(o_t + q * 32, v);
+              uint32_t o[32];
+              ptx::tmem_ld32(o_t + q * 32, o);
               ptx::tmem_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 32; i++) v[i] = __float_as_uint(__uint_as_float(v[i]) * a);
-              ptx::tmem_st32(o_t + q * 32, v);
+              for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              ptx::tmem_st32(o_t + q * 32, o);
             }
           }
+          vrun = vn;
         }
-        const float mc = m == -INFINITY ? 0.f : m * c;
+        // P times 2^(kPreBits + ve - vrun)
+        const float add = kPreBits + (float)(ve - vrun);
+        const float mc = (m == -INFINITY ? 0.f : -m) + add;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int q = 0; q < 4; q++) {
-          ptx::tmem_ld32(s_t + q * 32, v);
-          ptx::tmem_wait_ld();
           uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 16; i++) {
-            float a = ex2(fmaf(__uint_as_float(v[2 * i]), c, -mc)), b = ex2(fmaf(__uint_as_float(v[2 * i + 1]), c, -mc));
-            if (masked) {
-              if (key0 + q * 32 + 2 * i > pos) a = 0.f;
-              if (key0 + q * 32 + 2 * i + 1 > pos) b = 0.f;
-            }
-            l += a + b;
-            pk[i] = ptx::pack_bf16x2(a, b);
+            const float a = ex2(fmaf(__uint_as_float(v[q * 32 + 2 * i]), c, mc));
+            const float b = ex2(fmaf(__uint_as_float(v[q * 32 + 2 * i + 1]), c, mc));
+            sum[i & 3] += a + b;
+            const __half2 h = __floats2half2_rn(a, b);
+            pk[i] = *reinterpret_cast<const uint32_t*>(&h);
           }
           ptx::tmem_st16(s_t + q * 16, pk);  // P over the columns of S already read
         }
         ptx::tmem_wait_st();
         ptx::tc_fence_before();
         ptx::mbar_arrive(&p_full[t]);
+        l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), ex2(-add), l);
       }
       if (ok) ok = __all_sync(0xffffffffu, ptx::mbar_wait(&o_full[t], items & 1));
       if (!ok) break;
       items++;
       ptx::tc_fence_after();
-      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+      const float unit = pre_pow2(vrun - kTop - (int)kPreBits);
+      const float inv = l > 0.f || l != l ? unit / l : 0.f;
       const int64_t part = (row * p.hq + it.head * p.G + head) * (int64_t)p.max_splits + it.split;
 #pragma unroll
       for (int q = 0; q < D / 32; q++) {
@@ -443,11 +523,15 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
           }
         } else {
 #pragma unroll
-          for (int u = 0; u < 8; u++)
-            reinterpret_cast<uint4*>(p.part_o + part * D)[q * 8 + u] = make_uint4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+          for (int u = 0; u < 8; u++) {
+            float4 f;
+            f.x = __uint_as_float(v[4 * u]) * unit, f.y = __uint_as_float(v[4 * u + 1]) * unit;
+            f.z = __uint_as_float(v[4 * u + 2]) * unit, f.w = __uint_as_float(v[4 * u + 3]) * unit;
+            reinterpret_cast<float4*>(p.part_o + part * D)[q * 8 + u] = f;
+          }
         }
       }
-      if (real && ns > 1) p.part_ml[2 * part] = m * c, p.part_ml[2 * part + 1] = l;
+      if (real && ns > 1) p.part_ml[2 * part] = m, p.part_ml[2 * part + 1] = l;
       ptx::tc_fence_before();
     }
     if (!ok) s_fail = 1;

@@ -338,6 +338,10 @@ ES_DEVICE bool named_bar_or(int id, int count, bool pred) {
   return r != 0;
 }
 
+// Instruction descriptor of tcgen05.mma kind::f16: f16 A and B, both K-major, fp32 D, M x N.
+__host__ __device__ constexpr uint32_t idesc_f16_f32(int m, int n) {
+  return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
 // Instruction descriptor of tcgen05.mma kind::f16: bf16 A and B, both K-major, fp32 D, M x N.
 __host__ __device__ constexpr uint32_t idesc_bf16_f32(int m, int n) {
   return (1u << 4)                       // D format: f32

@@ -4,7 +4,8 @@ Blocks are fixed-size runs of ``block_size`` token slots. A request owns a list 
 block table); token position p lives at slot ``blocks[p // block_size] * block_size + p %
 block_size``. Free blocks are handed out lowest id first, so two engines that see the same request
 sequence lay their caches out identically (a spare's restore writes to the slots the lost rank
-used).
+used). Requests forked from one another hold their common full blocks together: a block is free
+again when the last request holding it gives it back.
 """
 
 from __future__ import annotations
@@ -19,6 +20,7 @@ class BlockManager:
         self.block_size = block_size
         self._free = list(range(num_blocks))
         heapq.heapify(self._free)
+        self._shared: dict[int, int] = {}  # holders of a block beyond the first
 
     @property
     def free_blocks(self) -> int:
@@ -40,8 +42,20 @@ class BlockManager:
 
     def free(self, blocks: list[int]) -> None:
         for b in blocks:
-            heapq.heappush(self._free, b)
+            n = self._shared.get(b, 0)
+            if n == 0:
+                heapq.heappush(self._free, b)
+            elif n == 1:
+                del self._shared[b]
+            else:
+                self._shared[b] = n - 1
         blocks.clear()
+
+    def share(self, blocks: list[int]) -> list[int]:
+        """The same blocks, held once more (each holder frees its own list)."""
+        for b in blocks:
+            self._shared[b] = self._shared.get(b, 0) + 1
+        return list(blocks)
 
     def take(self, ids: list[int]) -> None:
         """Mark specific blocks used (a restore that must reproduce another engine's layout)."""

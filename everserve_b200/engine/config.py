@@ -29,6 +29,11 @@ class EngineConfig:
     # "fp8": the dense projections' weights in e4m3 with one scale per 128 x 128 block, activations
     # quantized per token and 128-wide block (the block-scaled fp8 GEMM); None: bf16
     quant: str | None = None
+    # "int4": the K/V cache in 4 bits, a bf16 scale and zero per token and `kv_group` channels (64, or
+    # 0: the whole head), 3.6 times the positions in the same memory; None: the model's dtype. The
+    # committed-KV store and multi-process executors take the unquantized cache only
+    kv_quant: str | None = None
+    kv_group: int = 64
     # tensor-parallel ranks keep the residual stream of their token slice (norms on the slice,
     # reduce-scatter GEMMs for o/down, all-gather GEMMs for qkv/gate_up/vocabulary); ES_SP=1 sets it
     sequence_parallel: bool = field(default_factory=lambda: os.environ.get("ES_SP", "0") == "1")
@@ -49,6 +54,13 @@ class EngineConfig:
             raise ValueError("block_size must be 16 or 32")
         if self.quant not in (None, "fp8"):
             raise ValueError(f"unknown quantization {self.quant!r}")
+        if self.kv_quant not in (None, "int4"):
+            raise ValueError(f"unknown K/V cache quantization {self.kv_quant!r}")
+        if self.kv_quant == "int4":
+            if self.model.head_dim not in (64, 128):
+                raise ValueError("a 4-bit K/V cache needs a head dim of 64 or 128")
+            if self.kv_group not in (0, 64, self.model.head_dim):
+                raise ValueError(f"kv_group must be 64 or 0 (the whole head), got {self.kv_group}")
 
     @property
     def world_size(self) -> int:

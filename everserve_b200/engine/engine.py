@@ -61,6 +61,9 @@ class LocalExecutor:
     def decode_loop(self, plan: StepPlan, k: int, after_step=None):
         return self.worker.runner.decode_loop(plan, k, after_step)
 
+    def copy_pages(self, pairs: list[tuple[int, int]]) -> None:
+        self.worker.runner.copy_pages(pairs)
+
     # pipelined decode (Engine.step keeps one step in flight): see ModelRunner.launch_next
     def launch_next(self, plan: StepPlan, prev_ids):
         return self.worker.runner.launch_next(plan, prev_ids)
@@ -88,7 +91,10 @@ class Engine:
         self.executor = executor if executor is not None else LocalExecutor(cfg)
         self.blocks = BlockManager(self.executor.num_blocks, cfg.block_size)
         self.scheduler = Scheduler(self.blocks, cfg.max_batch, cfg.max_prefill_tokens, cfg.max_model_len)
+        if connector is not None and cfg.kv_quant is not None:
+            raise ValueError("the committed-KV store takes the unquantized K/V cache only")
         self.connector = connector
+        self._early: list[tuple[str, int | None, bool]] = []  # results a fork applied, for the next step()
         self.step_fn: Callable[[], list] = self._step
         self.last_plan: StepPlan | None = None
         self._ahead: _InFlight | None = None
@@ -103,10 +109,32 @@ class Engine:
         return req.req_id
 
     def has_work(self) -> bool:
-        return self.scheduler.has_work() or self._ahead is not None
+        return self.scheduler.has_work() or self._ahead is not None or bool(self._early)
 
     def request(self, req_id: str) -> Request:
         return self.scheduler.requests[req_id]
+
+    def fork(self, req_id: str, params: SamplingParams | None = None, keep: int | None = None,
+             new_id: str | None = None) -> str:
+        """Continue a running request a second time: a new request with its first `keep` tokens (default:
+        all so far; its prompt's length draws every output anew) and its own `params` (default: the
+        request's). Nothing is recomputed: the two hold the full cache blocks of the common tokens
+        together, and the block the new one writes into is copied. Call it between steps."""
+        if not hasattr(self.executor, "copy_pages"):
+            raise NotImplementedError("this executor does not copy cache blocks")
+        if self.connector is not None:
+            raise ValueError("a request whose cache is committed to a store cannot be forked")
+        parent = self.scheduler.requests[req_id]
+        self._early += self.flush()
+        keep = parent.num_tokens if keep is None else keep
+        if not 1 <= keep <= parent.num_tokens:
+            raise ValueError(f"keep must be 1 .. {parent.num_tokens}, got {keep}")
+        n = min(keep, len(parent.prompt))
+        req = Request(parent.prompt[:n], params or parent.params, outputs=parent.outputs[: keep - n])
+        if new_id is not None:
+            req.req_id = new_id
+        self.executor.copy_pages(self.scheduler.fork(parent, req, keep))
+        return req.req_id
 
     # ---- stepping --------------------------------------------------------------------------------
     def wrap_step(self, wrapper: Callable[[Callable[[], list]], Callable[[], list]]) -> None:
@@ -114,6 +142,9 @@ class Engine:
         self.step_fn = wrapper(self.step_fn)
 
     def step(self) -> list[tuple[str, int | None, bool]]:
+        if self._early:
+            early, self._early = self._early, []
+            return early + self.step_fn()
         return self.step_fn()
 
     def _step(self) -> list[tuple[str, int | None, bool]]:
@@ -264,6 +295,28 @@ class Engine:
     def generate(self, prompts: list[list[int]], max_tokens: int = 16, **sampling) -> list[list[int]]:
         """Every prompt to completion; `sampling`: temperature, top_k, top_p, seed (greedy by default)."""
         ids = [self.add_request(p, SamplingParams(max_tokens=max_tokens, **sampling)) for p in prompts]
+        while self.has_work():
+            self.step()
+        return [self.scheduler.requests[i].outputs for i in ids]
+
+    def samples(self, prompt: list[int], n: int, max_tokens: int = 16, **sampling) -> list[list[int]]:
+        """n completions of one prompt, which is prefilled once: the others are forked from it. `sampling`
+        as in `generate`; with a seed, completion i takes seed + i."""
+        if n < 1:
+            raise ValueError("n must be at least 1")
+        seed = sampling.pop("seed", None)
+        each = [SamplingParams(max_tokens=max_tokens, seed=None if seed is None else seed + i, **sampling) for i in range(n)]
+        first = self.add_request(prompt, each[0])
+        req = self.scheduler.requests[first]
+        while not req.outputs:
+            self.step()
+        ids = [first]
+        for p in each[1:]:
+            # a batch without room, or a request that ended meanwhile: the prompt by itself
+            if req.status is Status.RUNNING and len(self.scheduler.running) < self.cfg.max_batch and self.blocks.free_blocks:
+                ids.append(self.fork(first, p, keep=len(prompt)))
+            else:
+                ids.append(self.add_request(prompt, p))
         while self.has_work():
             self.step()
         return [self.scheduler.requests[i].outputs for i in ids]

@@ -19,7 +19,7 @@ from __future__ import annotations
 import torch
 
 from ..models.llama import DecoderLM, StepInput
-from ..ops import prefill_tiles
+from ..ops import check_pairs, prefill_tiles
 from .sampling import SamplingBatch
 from .scheduler import StepPlan
 
@@ -38,7 +38,7 @@ class ModelRunner:
         self.max_blocks = (max_model_len + block_size - 1) // block_size
         self.use_graphs = use_graphs and self.device.type == "cuda"
         shape = model.kv_cache_shape(num_blocks, block_size)
-        self.caches = [torch.zeros(shape, dtype=model.dtype, device=self.device) for _ in range(model.l1 - model.l0)]
+        self.caches = [torch.zeros(shape, dtype=model.kv_dtype, device=self.device) for _ in range(model.l1 - model.l0)]
         self.buckets = [b for b in _BUCKETS if b < max_batch] + [max_batch]
         B = max_batch
         pin = self.device.type == "cuda"
@@ -183,10 +183,21 @@ class ModelRunner:
             ps = [r.sampling or (0.0, 0, 1.0, 0) for r in plan.reqs]
             sb = SamplingBatch(temperature=t([p[0] for p in ps], torch.float32), top_k=t([p[1] for p in ps]),
                                top_p=t([p[2] for p in ps], torch.float32), seed=t([p[3] for p in ps]))
-        tiles = prefill_tiles(seq, pos, device=dev) if self.model.ops.kind == "kernel" else None
+        plan_tiles = self.model.ops.kind == "kernel" and self.model.kv_quant is None
+        tiles = prefill_tiles(seq, pos, device=dev) if plan_tiles else None
         return StepInput(ids=t(ids), positions=t(pos), slots=t(slots), block_tables=bt.to(dev),
                          ctx_lens=t(ctx, torch.int32), q_seq=t(seq), logits_idx=t(last), is_decode=False,
-                         max_model_len=self.max_model_len, sampling=sb, prefill_tiles=tiles)
+                         max_model_len=self.max_model_len, sampling=sb, prefill_tiles=tiles, max_context=max(ctx))
+
+    def copy_pages(self, pairs: list[tuple[int, int]]) -> None:
+        """Copy blocks (from, to) in every layer's cache, behind the work enqueued so far."""
+        if not pairs:
+            return
+        p = torch.tensor(pairs, dtype=torch.int64)
+        check_pairs(p)
+        if self.device.type == "cuda":
+            p = p.pin_memory().to(self.device, non_blocking=True)
+        self.model.ops.copy_pages(self.caches, p)
 
     # ---- forward ---------------------------------------------------------------------------------
     def forward(self, inp: StepInput, hidden=None, residual=None):

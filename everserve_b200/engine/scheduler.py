@@ -77,6 +77,36 @@ class Scheduler:
         self.requests[req.req_id] = req
         self.waiting.append(req)
 
+    def fork(self, parent: Request, req: Request, keep: int) -> list[tuple[int, int]]:
+        """Start `req`, whose first `keep` tokens are the running `parent`'s, on the parent's cache: full
+        blocks of computed positions are held by both, the block it writes next becomes its own. Returns
+        the (from, to) blocks to copy before the next step."""
+        if parent.status is not Status.RUNNING:
+            raise ValueError(f"request {parent.req_id} is not running")
+        if req.req_id in self.requests:
+            raise ValueError(f"request {req.req_id} exists")
+        if len(self.running) >= self.max_batch:
+            raise RuntimeError("the batch is full")
+        if len(req.prompt) + req.params.max_tokens > self.max_model_len:
+            raise ValueError(f"request needs {len(req.prompt) + req.params.max_tokens} positions, "
+                             f"max_model_len is {self.max_model_len}")
+        done = min(parent.num_computed, keep - 1)
+        full, part = divmod(done, self.bm.block_size)
+        if part and self.bm.free_blocks < 1:
+            raise MemoryError("need 1 KV blocks, 0 free")
+        req.blocks = self.bm.share(parent.blocks[:full])
+        copies = []
+        if part:
+            self.bm.grow(req.blocks, done)
+            copies.append((parent.blocks[full], req.blocks[full]))
+        req.num_computed = done
+        req.status = Status.RUNNING
+        req.arrival = self._arrivals
+        self._arrivals += 1
+        self.requests[req.req_id] = req
+        self.running.append(req)
+        return copies
+
     def has_work(self) -> bool:
         return bool(self.waiting or self.running)
 

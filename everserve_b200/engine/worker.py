@@ -40,7 +40,8 @@ class Worker:
         init = "none" if (cfg.checkpoint or weights is not None) else "random"
         self.model = DecoderLM(cfg.model, self.device, cfg.dtype, cfg.seed, self.tp, layers, init=init,
                                quant=getattr(cfg, "quant", None),
-                               sequence_parallel=getattr(cfg, "sequence_parallel", False))
+                               sequence_parallel=getattr(cfg, "sequence_parallel", False),
+                               kv_quant=getattr(cfg, "kv_quant", None), kv_group=getattr(cfg, "kv_group", 64))
         if weights is not None:  # a resident copy (pinned host memory): copied in, no init
             for k, t in weights.items():
                 self.model._put(k, t)

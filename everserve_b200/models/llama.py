@@ -17,6 +17,7 @@ group, which is the fused GEMM + all-reduce when the group has one.
 from __future__ import annotations
 
 import hashlib
+import math
 import os
 from dataclasses import dataclass
 
@@ -42,6 +43,7 @@ class StepInput:
     sampling: object | None = None  # engine.sampling.SamplingBatch of the rows; None: greedy
     logprobs_k: int | None = None  # the step also reports log-probabilities (k alternatives)
     prefill_tiles: torch.Tensor | None = None  # prefill kernel work list (ops.prefill_tiles), device
+    max_context: int | None = None  # the largest context length, where the host knows it
 
 
 def _seed_of(seed: int, *parts) -> int:
@@ -129,8 +131,12 @@ class DecoderLM:
 
     def __init__(self, cfg: ModelConfig, device="cpu", dtype=torch.bfloat16, seed: int = 0,
                  tp: TPGroup | None = None, layer_range: tuple[int, int] | None = None,
-                 init: str = "random", quant: str | None = None, sequence_parallel: bool = False):
+                 init: str = "random", quant: str | None = None, sequence_parallel: bool = False,
+                 kv_quant: str | None = None, kv_group: int = 64):
         self.cfg = cfg
+        # "int4": the cache in 4 bits, kv_group channels to a scale (0: the whole head)
+        self.kv_quant = kv_quant
+        self.kv_group = kv_group or cfg.head_dim
         # fp8: those weights stored as e4m3 with 128 x 128 block scales (key.q8, key.s8)
         self.fp8 = quant == "fp8"
         if self.fp8 and cfg.is_moe:
@@ -178,7 +184,7 @@ class DecoderLM:
                            and os.environ.get("ES_FUSED_SILU", "1") != "0")
         # the qkv GEMM's RoPE + KV-write epilogue (kernels, bf16, head dim 128, no qkv bias)
         self.fused_rope = (self.ops.kind == "kernel" and not self.fp8 and cfg.head_dim == 128
-                           and not cfg.qkv_bias and os.environ.get("ES_FUSED_ROPE", "1") != "0")
+                           and not cfg.qkv_bias and kv_quant is None and os.environ.get("ES_FUSED_ROPE", "1") != "0")
         self.packed_weights = (self.ops.kind == "kernel" and not cfg.is_moe
                                and os.environ.get("ES_PACK_WEIGHTS", "1") != "0")
         self.cos_sin = ref.cos_sin_table(cfg.head_dim, cfg.max_position, cfg.rope_theta, cfg.rope_scaling).to(self.device)
@@ -281,10 +287,35 @@ class DecoderLM:
 
     # ---- KV cache ------------------------------------------------------------------------------
     def kv_cache_shape(self, num_blocks: int, block_size: int) -> tuple[int, ...]:
+        if self.kv_quant is not None:
+            return ref.kv4_cache_shape(num_blocks, self.hkv, block_size, self.d, self.kv_group)
         return (num_blocks, 2, self.hkv, block_size, self.d)
 
+    @property
+    def kv_dtype(self) -> torch.dtype:
+        return torch.uint8 if self.kv_quant is not None else self.dtype
+
     def bytes_per_block(self, block_size: int) -> int:
-        return 2 * self.hkv * block_size * self.d * torch.tensor([], dtype=self.dtype).element_size() * (self.l1 - self.l0)
+        return math.prod(self.kv_cache_shape(1, block_size)) * self.kv_dtype.itemsize * (self.l1 - self.l0)
+
+    def block_size_of(self, cache: torch.Tensor) -> int:
+        """Positions of a block of one of ``kv_cache_shape``'s caches."""
+        if self.kv_quant is not None:
+            return cache.shape[2] // (self.d + 8 * (self.d // self.kv_group))
+        return cache.shape[3]
+
+    def _write_kv(self, ops, qkv, bias, inp: StepInput, cache, bs: int):
+        """RoPE and the write of the step's rows into the layer's cache; returns q."""
+        write = ops.rope_kv_write if self.kv_quant is None else ops.rope_kv4_write
+        return write(qkv, bias, inp.positions, self.cos_sin, inp.slots, cache, self.hq, self.hkv, bs)
+
+    def _attend_kv4(self, ops, q, cache, inp: StepInput, bs: int):
+        """Attention of the step's rows over a cache in 4 bits."""
+        if inp.is_decode:
+            return ops.decode_attention_kv4(q, cache, inp.block_tables, inp.ctx_lens, self.scale, bs,
+                                            inp.max_model_len or None)
+        return ops.prefill_attention_kv4(q, cache, inp.block_tables, inp.ctx_lens, inp.logits_idx, self.scale, bs,
+                                         inp.max_context)
 
     # ---- forward -------------------------------------------------------------------------------
     def embed(self, ids: torch.Tensor) -> torch.Tensor:
@@ -310,7 +341,7 @@ class DecoderLM:
             h = ops.rmsnorm(x, W[f"l{self.l0}.in_norm"], c.rms_eps)
         else:
             h = ops.rmsnorm(hidden, W[f"l{self.l0}.in_norm"], c.rms_eps, residual)
-        bs = caches[0].shape[3] if caches else 16
+        bs = self.block_size_of(caches[0]) if caches else 16
         for i, l in enumerate(range(self.l0, self.l1)):
             p = f"l{l}."
             cache = caches[i]
@@ -320,9 +351,10 @@ class DecoderLM:
                                        self.hq, self.hkv, bs)
             else:
                 qkv = self._linear(ops, h, p + "qkv")
-                q = ops.rope_kv_write(qkv, W.get(p + "qkv_bias"), inp.positions, self.cos_sin, inp.slots, cache,
-                                      self.hq, self.hkv, bs)
-            if inp.is_decode:
+                q = self._write_kv(ops, qkv, W.get(p + "qkv_bias"), inp, cache, bs)
+            if self.kv_quant is not None:
+                a = self._attend_kv4(ops, q, cache, inp, bs)
+            elif inp.is_decode:
                 if ops.kind == "kernel":
                     # the attention streams the history; meanwhile it brings o_proj's weights into L2
                     a = ops.decode_attention(q, cache, inp.block_tables, inp.ctx_lens, self.scale,
@@ -380,15 +412,16 @@ class DecoderLM:
         residual = torch.zeros(per, c.hidden, dtype=x.dtype, device=x.device)
         residual[: hi - lo] = x[lo:hi]
         h = ops.rmsnorm(residual, W[f"l{self.l0}.in_norm"], c.rms_eps)
-        bs = caches[0].shape[3] if caches else 16
+        bs = self.block_size_of(caches[0]) if caches else 16
         hidden = None
         for i, l in enumerate(range(self.l0, self.l1)):
             p = f"l{l}."
             cache = caches[i]
             qkv = self.tp.gather_linear(ops, h, W[p + "qkv"])[:M]  # the first M rows: contiguous
-            q = ops.rope_kv_write(qkv, W.get(p + "qkv_bias"), inp.positions, self.cos_sin, inp.slots, cache,
-                                  self.hq, self.hkv, bs)
-            if inp.is_decode:
+            q = self._write_kv(ops, qkv, W.get(p + "qkv_bias"), inp, cache, bs)
+            if self.kv_quant is not None:
+                a = self._attend_kv4(ops, q, cache, inp, bs)
+            elif inp.is_decode:
                 if ops.kind == "kernel":
                     # the attention streams the history; meanwhile it brings o_proj's weights into L2
                     a = ops.decode_attention(q, cache, inp.block_tables, inp.ctx_lens, self.scale,

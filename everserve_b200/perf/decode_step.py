@@ -22,17 +22,25 @@ from ..models.config import get_config
 from ..models.llama import DecoderLM, StepInput
 
 
-def build(model: str, batch: int, ctx: int, layers: int | None, bs: int = 16, seed: int = 0, tp=None):
+def build(model: str, batch: int, ctx: int, layers: int | None, bs: int = 16, seed: int = 0, tp=None,
+          kv_quant: str | None = None):
     cfg = get_config(model)
     if layers:
         cfg = dataclasses.replace(cfg, layers=layers)
     dev = torch.device("cuda", torch.cuda.current_device())
-    m = DecoderLM(cfg, dev, torch.bfloat16, seed, tp=tp)
+    m = DecoderLM(cfg, dev, torch.bfloat16, seed, tp=tp, kv_quant=kv_quant)
     max_len = ctx + 64
     mb = (max_len + bs - 1) // bs
     nb = batch * mb
     g = torch.Generator(device=dev).manual_seed(seed)
-    caches = [torch.randn(m.kv_cache_shape(nb, bs), generator=g, device=dev).bfloat16() for _ in range(cfg.layers)]
+    if kv_quant is None:
+        caches = [torch.randn(m.kv_cache_shape(nb, bs), generator=g, device=dev).bfloat16() for _ in range(cfg.layers)]
+    else:  # quantized rows of one random layer, in every layer
+        one = torch.zeros(m.kv_cache_shape(nb, bs), dtype=m.kv_dtype, device=dev)
+        rows = torch.randn(nb * bs, (m.hq + 2 * m.hkv) * m.d, generator=g, device=dev).bfloat16()
+        at = torch.arange(nb * bs, device=dev)
+        m.ops.rope_kv4_write(rows, None, at % cfg.max_position, m.cos_sin, at, one, m.hq, m.hkv, bs)
+        caches = [one.clone() for _ in range(cfg.layers)]
     bt = torch.arange(nb, device=dev, dtype=torch.int32).view(batch, mb)
     pos = torch.full((batch,), ctx, device=dev, dtype=torch.int64)
     slots = bt[:, ctx // bs].long() * bs + ctx % bs
@@ -55,6 +63,7 @@ def main() -> None:
     ap.add_argument("--eager", action="store_true")
     ap.add_argument("--collective", default="fused", choices=["fused", "nccl"])
     ap.add_argument("--breakdown", action="store_true")
+    ap.add_argument("--kv-quant", default=None, choices=["int4"])
     a = ap.parse_args()
     import os
 
@@ -75,7 +84,7 @@ def main() -> None:
         dist.init_process_group("nccl", device_id=torch.device("cuda", local), timeout=timedelta(seconds=120))
         coll = make_tp_collective(torch.device("cuda", local), kind=a.collective)
         tp = TPGroup(rank, world, coll)
-    m, caches, inp = build(a.model, a.batch, a.ctx, a.layers, tp=tp)
+    m, caches, inp = build(a.model, a.batch, a.ctx, a.layers, tp=tp, kv_quant=a.kv_quant)
     fwd = lambda: m.forward(inp, caches)  # noqa: E731
     for _ in range(2):
         fwd()
@@ -100,7 +109,7 @@ def main() -> None:
         dist.all_reduce(t, op=dist.ReduceOp.MAX)
         ms = float(t.item())
     w_bytes = sum(w.numel() * w.element_size() for w in m.weights.values())
-    kv_bytes = a.batch * (a.ctx + 1) * 2 * m.hkv * m.d * 2 * (m.l1 - m.l0)
+    kv_bytes = a.batch * (a.ctx + 1) * m.bytes_per_block(16) // 16
     if rank != 0:
         pass
     else:

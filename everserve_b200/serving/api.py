@@ -211,10 +211,11 @@ def main(argv=None) -> int:
     ap.add_argument("--port", type=int, default=8000)
     ap.add_argument("--max-batch", type=int, default=64)
     ap.add_argument("--max-model-len", type=int, default=4096)
+    ap.add_argument("--kv-quant", default=None, choices=["int4"], help="hold the K/V cache in 4 bits")
     a = ap.parse_args(argv)
     dtype = torch.bfloat16 if a.device.startswith("cuda") else torch.float32
     cfg = EngineConfig(a.model, device=a.device, dtype=dtype, max_batch=a.max_batch, max_model_len=a.max_model_len,
-                       checkpoint=a.checkpoint)
+                       checkpoint=a.checkpoint, kv_quant=a.kv_quant)
     tok = None
     if a.tokenizer:
         from transformers import AutoTokenizer

@@ -105,6 +105,8 @@ class MultiprocExecutor:
         and store sockets and the node name ({"daemon": ..., "store": ..., "node": ...}).
         `local_ranks`: the ranks this head starts itself (default: all); node agents
         (``everserve_b200.serving.node``) start the others on their nodes."""
+        if cfg.kv_quant is not None:
+            raise ValueError("the multi-process executor's ranks hold the unquantized K/V cache only")
         self.cfg = cfg
         self.engine = engine
         self._closed = False

@@ -1,0 +1,119 @@
+"""The engine on a 4-bit K/V cache and forked requests, on the CPU's reference ops."""
+
+import pytest
+import torch
+
+from everserve_b200.engine import Engine, EngineConfig, SamplingParams
+from everserve_b200.engine.block_manager import BlockManager
+from everserve_b200.models.config import LLAMA3_8B, TINY_LLAMA, TINY_MIXTRAL, TINY_QWEN
+from everserve_b200.models.llama import DecoderLM
+
+
+def _engine(model=TINY_LLAMA, **kw):
+    args = dict(device="cpu", dtype=torch.float32, max_batch=4, max_model_len=256, num_blocks=64)
+    args.update(kw)
+    return Engine(EngineConfig(model, **args))
+
+
+@pytest.mark.parametrize("model", [TINY_LLAMA, TINY_QWEN, TINY_MIXTRAL])
+def test_generate_on_4_bits(model):
+    """Decoding from the cache predicts what a prefill of the same tokens predicts."""
+    prompt = [(7 * i + 3) % 500 for i in range(40)]
+    eng = _engine(model, kv_quant="int4")
+    assert eng.executor.worker.runner.caches[0].dtype == torch.uint8
+    out = eng.generate([prompt, prompt[:9]], max_tokens=6)
+    again = _engine(model, kv_quant="int4").generate([prompt + out[0][:-1]], max_tokens=1)
+    assert again[0] == [out[0][-1]]
+
+
+def test_memory_of_a_block():
+    def model(**kw):
+        return DecoderLM(LLAMA3_8B, "cpu", torch.bfloat16, layer_range=(0, 1), init="none", **kw)
+
+    dense, int4, whole = (model(**kw).bytes_per_block(16) for kw in ({}, {"kv_quant": "int4"}, {"kv_quant": "int4", "kv_group": 0}))
+    assert (dense, int4, whole) == (16 * 8 * 512, 16 * 8 * 144, 16 * 8 * 136)
+
+
+def test_config_refused():
+    for kw in (dict(kv_quant="int3"), dict(kv_quant="int4", kv_group=32)):
+        with pytest.raises(ValueError):
+            EngineConfig(TINY_LLAMA, device="cpu", **kw)
+    with pytest.raises(ValueError):
+        Engine(EngineConfig(TINY_LLAMA, device="cpu", dtype=torch.float32, num_blocks=8, kv_quant="int4"), connector=object())
+    from everserve_b200.serving.executor import MultiprocExecutor
+
+    with pytest.raises(ValueError):
+        MultiprocExecutor(EngineConfig(TINY_LLAMA, device="cpu", kv_quant="int4"))
+
+
+def test_shared_blocks():
+    bm = BlockManager(4, 16)
+    a = []
+    bm.grow(a, 33)
+    b, c = bm.share(a[:2]), bm.share(a[:1])
+    bm.free(a)
+    assert bm.free_blocks == 2 and b == [0, 1]
+    bm.free(b)
+    assert bm.free_blocks == 3 and c == [0]
+    bm.free(c)
+    assert bm.free_blocks == 4
+    d = []
+    bm.grow(d, 64)
+    assert d == [0, 1, 2, 3]
+
+
+@pytest.mark.parametrize("kv", [None, "int4"])
+@pytest.mark.parametrize("plen", [1, 16, 17, 31, 40])
+def test_samples_are_their_seeds_own_runs(kv, plen):
+    """Forked completions draw what the same prompt and seed draw by themselves."""
+    prompt = [(5 * i + 2) % 500 for i in range(plen)]
+    kw = dict(max_tokens=20, temperature=0.9, top_k=20)
+    eng = _engine(kv_quant=kv)
+    got = eng.samples(prompt, 3, seed=11, **kw)
+    assert eng.blocks.free_blocks == 64
+    alone = [_engine(kv_quant=kv).generate([prompt], seed=11 + i, **kw)[0] for i in range(3)]
+    assert got == alone and got[0] != got[1]
+
+
+def test_fork_mid_way():
+    """A fork of a request under way continues as the request does; one from an earlier token replays it;
+    results the fork had to apply come with the next step."""
+    eng = _engine()
+    rid = eng.add_request([3, 1, 4, 1, 5, 9, 2, 6, 5, 3, 5, 8, 9, 7, 9, 3, 2, 3, 8], SamplingParams(max_tokens=24))
+    seen = []
+    for _ in range(8):
+        seen += eng.step()
+    twin = eng.fork(rid)
+    back = eng.fork(rid, keep=21)
+    while eng.has_work():
+        seen += eng.step()
+    out = eng.request(rid).outputs
+    assert len(out) == 24 and eng.request(twin).outputs == out and eng.request(back).outputs == out
+    assert [t for r, t, _ in seen if r == rid] == out
+    assert eng.blocks.free_blocks == 64
+    with pytest.raises(ValueError):
+        eng.fork(rid)  # finished
+    with pytest.raises(KeyError):
+        eng.fork("nobody")
+
+
+def test_fork_limits_and_preemption():
+    eng = _engine(max_batch=2, num_blocks=8)
+    rid = eng.add_request(list(range(1, 40)), SamplingParams(max_tokens=40))
+    eng.step()
+    for keep in (0, 41):
+        with pytest.raises(ValueError):
+            eng.fork(rid, keep=keep)
+    twin = eng.fork(rid)
+    with pytest.raises(RuntimeError):
+        eng.fork(rid)
+    want = _engine().generate([list(range(1, 40))], max_tokens=40)[0]
+    while eng.has_work():  # 8 blocks do not hold both to the end: one is preempted and recomputed
+        eng.step()
+    assert eng.request(rid).outputs == want and eng.request(twin).outputs == want
+    assert eng.blocks.free_blocks == 8
+    tight = _engine(num_blocks=3)
+    rid = tight.add_request(list(range(1, 40)), SamplingParams(max_tokens=2))
+    tight.step()
+    with pytest.raises(MemoryError):
+        tight.fork(rid)
