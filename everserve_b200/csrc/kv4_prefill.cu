@@ -137,6 +137,11 @@ ES_DEVICE bool find_item(const PreParams& p, int bs, int idx, Item& it) {
   return false;
 }
 
+// A CTA's item of a round: every other round the other way, as an item's length falls along the order.
+ES_DEVICE int item_of(int round) {
+  return round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+}
+
 // The key tiles [j0, j1) of an item, and how many items its row tile has.
 ES_DEVICE void span(const PreParams& p, const Item& it, int& j0, int& j1, int& ns) {
   const int last = min(it.rows, (it.tile + 1) * 2 * p.tt) - 1;  // the tile's last token
@@ -177,9 +182,17 @@ struct Raw {
   uint32_t km[kPer][NG], vm[kPer][NG];
 };
 
-// The i-th piece of key tile j.
+// The block of the key that a thread's i-th piece of key tile j belongs to (0 past the history).
+template <int D, int BS>
+ES_DEVICE int block_of(const PreParams& p, const Item& it, int j, int i, int tid) {
+  constexpr int P = D / 32;
+  const int key = j * kKeys + i * (kConvThreads / P) + tid / P;
+  return key < it.ctx ? p.block_tables[(int64_t)it.seq * p.bt_stride + key / BS] : 0;
+}
+
+// The i-th piece of key tile j, of block blk.
 template <int D, int NG, int BS>
-ES_DEVICE void load_raw(Raw<D, NG>& r, int i, const PreParams& p, const Item& it, int j, int tid) {
+ES_DEVICE void load_raw(Raw<D, NG>& r, int i, const PreParams& p, const Item& it, int j, int tid, int64_t blk) {
   using R = Rec<D, NG, BS>;
   constexpr int P = D / 32;
   const int key = j * kKeys + i * (kConvThreads / P) + tid / P;
@@ -187,7 +200,6 @@ ES_DEVICE void load_raw(Raw<D, NG>& r, int i, const PreParams& p, const Item& it
 #pragma unroll
   for (int g = 0; g < NG; g++) r.km[i][g] = r.vm[i][g] = 0;
   if (key < it.ctx) {
-    int64_t blk = p.block_tables[(int64_t)it.seq * p.bt_stride + key / BS];
     if (blk < 0 || blk >= p.num_blocks) {  // not a block of this cache: reported, block 0 read instead
       if (p.status) atomicExch(p.status, (int)kBadShape);
       blk = 0;
@@ -276,13 +288,19 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
     constexpr int P = D / 32;
     const int tid = threadIdx.x - kSoftThreads;
     uint32_t n = 0;  // key tiles converted so far, over all items
-    for (int idx = blockIdx.x; ok && find_item(p, BS, idx, it); idx += gridDim.x) {
+    for (int round = 0; ok && find_item(p, BS, item_of(round), it); round++) {
       span(p, it, j0, j1, ns);
       if (j0 >= j1) continue;
       Raw<D, NG> r;
       int vr = -100;  // the largest of V's exponents so far
+      int blk[P];     // the next tile's blocks: a table entry is asked for two tiles ahead, its data one
 #pragma unroll
-      for (int i = 0; i < P; i++) load_raw<D, NG, BS>(r, i, p, it, j0, tid);
+      for (int i = 0; i < P; i++) blk[i] = block_of<D, BS>(p, it, j0, i, tid);
+#pragma unroll
+      for (int i = 0; i < P; i++) {
+        load_raw<D, NG, BS>(r, i, p, it, j0, tid, blk[i]);
+        blk[i] = block_of<D, BS>(p, it, j0 + 1, i, tid);
+      }
       for (int j = j0; j < j1; j++, n++) {
         const int s = n & 1;
         uint32_t kb = 0, vb = 0;
@@ -311,7 +329,10 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
           const int row = i * (kConvThreads / P) + tid / P;
           store_piece<D, NG>(kt, row, tid % P, r.k[i], r.km[i], kf);
           store_piece<D, NG>(kt + C::kTile, row, tid % P, r.v[i], r.vm[i], vf);
-          if (j + 1 < j1) load_raw<D, NG, BS>(r, i, p, it, j + 1, tid);
+          if (j + 1 < j1) {
+            load_raw<D, NG, BS>(r, i, p, it, j + 1, tid, blk[i]);
+            blk[i] = block_of<D, BS>(p, it, j + 2, i, tid);
+          }
         }
         ptx::fence_proxy_async();
         ptx::mbar_arrive(&kv_full[s]);
@@ -324,58 +345,67 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
     ok = warp == 12;
     constexpr uint32_t idesc_s = ptx::idesc_f16_f32(kRows, kKeys);
     constexpr uint32_t idesc_o = ptx::idesc_f16_f32(kRows, D) | (1u << 16);  // V: MN-major
+    // The whole warp walks the loop, so that descriptors stay in uniform registers (a loop of one lane alone
+    // spent 150 cycles an MMA on moving them there: 770 us for the 8192-row prompt); one lane issues.
+    const bool leader = ptx::elect_one();
+    const uint64_t q_desc = ptx::sw128_kmajor_desc(ptx::smem_u32(q_s)), k_desc = ptx::sw128_kmajor_desc(ptx::smem_u32(kv_s));
+    const uint64_t v_desc = ptx::sw128_mnmajor_desc(ptx::smem_u32(kv_s + C::kTile), C::kChunk);
+    constexpr int kStageStep = 2 * C::kTile >> 4;
     uint32_t n = 0, items = 0;
     auto qk = [&](int t, int s) {  // S_t = Q_t . K^T
+      if (leader) {
+        const uint64_t a = q_desc + t * (C::kTile >> 4), b = k_desc + s * kStageStep;
 #pragma unroll
-      for (int kk = 0; kk < D / 16; kk++) {
-        const uint64_t a = ptx::sw128_kmajor_desc(ptx::smem_u32(q_s + t * C::kTile + (kk >> 2) * C::kChunk)) + 2 * (kk & 3);
-        const uint64_t b = ptx::sw128_kmajor_desc(ptx::smem_u32(kv_s + s * 2 * C::kTile + (kk >> 2) * C::kChunk)) + 2 * (kk & 3);
-        ptx::mma_f16_ss(tmem + t * 128, a, b, idesc_s, kk > 0 ? 1u : 0u);
+        for (int kk = 0; kk < D / 16; kk++) {
+          const int off = (kk >> 2) * (C::kChunk >> 4) + 2 * (kk & 3);
+          ptx::mma_f16_ss(tmem + t * 128, a + off, b + off, idesc_s, kk > 0 ? 1u : 0u);
+        }
+        ptx::mma_commit(&s_full[t]);
       }
-      ptx::mma_commit(&s_full[t]);
+      __syncwarp();
     };
-    for (int idx = blockIdx.x; ok && find_item(p, BS, idx, it); idx += gridDim.x) {
+    for (int round = 0; ok && find_item(p, BS, item_of(round), it); round++) {
       span(p, it, j0, j1, ns);
       if (j0 >= j1) continue;
-      if (lane == 0) {
-        ok = ptx::mbar_wait(&kv_full[n & 1], (n >> 1) & 1);
-        for (int t = 0; ok && t < 2; t++) {
-          ok = ptx::mbar_wait(&q_full[t], items & 1);
+      ok = __all_sync(0xffffffffu, ptx::mbar_wait(&kv_full[n & 1], (n >> 1) & 1));
+      for (int t = 0; ok && t < 2; t++) {
+        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&q_full[t], items & 1));
+        if (!ok) break;
+        ptx::tc_fence_after();
+        qk(t, n & 1);
+      }
+      for (int j = j0; ok && j < j1; j++, n++) {
+        const int s = n & 1;
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+          ok = ok && __all_sync(0xffffffffu, ptx::mbar_wait(&p_full[t], n & 1));
           if (!ok) break;
           ptx::tc_fence_after();
-          qk(t, n & 1);
-        }
-        for (int j = j0; ok && j < j1; j++, n++) {
-          const int s = n & 1;
-          const uint8_t* vt = kv_s + s * 2 * C::kTile + C::kTile;
-          for (int t = 0; ok && t < 2; t++) {
-            ok = ptx::mbar_wait(&p_full[t], n & 1);
-            if (!ok) break;
-            ptx::tc_fence_after();
+          if (leader) {
+            const uint64_t b = v_desc + s * kStageStep;
 #pragma unroll
             for (int kk = 0; kk < kKeys / 16; kk++)
-              ptx::mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8,
-                              ptx::sw128_mnmajor_desc(ptx::smem_u32(vt + kk * 16 * 128), C::kChunk), idesc_o,
+              ptx::mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, b + kk * (16 * 128 >> 4), idesc_o,
                               (j > j0 || kk > 0) ? 1u : 0u);
             if (t == 1) ptx::mma_commit(&kv_empty[s]);
-            if (j + 1 < j1) {
-              if (t == 0) ok = ptx::mbar_wait(&kv_full[s ^ 1], ((n + 1) >> 1) & 1);
-              if (!ok) break;
-              ptx::tc_fence_after();
-              qk(t, s ^ 1);  // after P_t . V in the tensor core's order, which P_t's columns wait for
-            } else {
-              ptx::mma_commit(&o_full[t]);
-            }
+            if (j + 1 == j1) ptx::mma_commit(&o_full[t]);
+          }
+          __syncwarp();
+          if (j + 1 < j1) {
+            if (t == 0) ok = __all_sync(0xffffffffu, ptx::mbar_wait(&kv_full[s ^ 1], ((n + 1) >> 1) & 1));
+            if (!ok) break;
+            ptx::tc_fence_after();
+            qk(t, s ^ 1);  // after P_t . V in the tensor core's order, which P_t's columns wait for
           }
         }
-        items++;
       }
-      ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+      items++;
     }
-    if (warp == 12 && lane == 0) {
+    if (warp == 12) {
       if (!ok) s_fail = 1;
-      ptx::mma_commit(mma_done);  // nothing of this CTA is in flight past here
-      ptx::mbar_wait(mma_done, 0);
+      if (leader) ptx::mma_commit(mma_done);
+      __syncwarp();
+      ptx::mbar_wait(mma_done, 0);  // nothing of this CTA is in flight past here
     }
   } else {
     // ---- softmax --------------------------------------------------------------------------------
@@ -384,9 +414,13 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
     const int r = threadIdx.x & 127;  // row of the tile (TMEM lane)
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_t = tmem + t * 128 + lane_base, o_t = tmem + 256 + t * 128 + lane_base;
-    const int token = r / p.G, head = r - token * p.G;
+    const int inv_g = (65536 + p.G - 1) / p.G;  // x / G = (x * inv_g) >> 16 for x < 128
+    const int token = (r * inv_g) >> 16, head = r - token * p.G;
     uint32_t n = 0, items = 0;
-    for (int idx = blockIdx.x; ok && find_item(p, BS, idx, it); idx += gridDim.x) {
+    Item nxt;
+    bool more = find_item(p, BS, item_of(0), nxt);
+    for (int round = 1; ok && more; round++) {
+      it = nxt;
       span(p, it, j0, j1, ns);
       const int tok0 = it.tile * 2 * p.tt + t * p.tt;  // the tile's first token of the sequence
       const int at = tok0 + token;
@@ -398,40 +432,52 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
       if (j0 >= j1) {
         if (it.split == 0 && real)  // no key at all
           for (int i = 0; i < D / 8; i++) reinterpret_cast<uint4*>(out)[i] = make_uint4(0, 0, 0, 0);
+        more = find_item(p, BS, item_of(round), nxt);
         continue;
       }
       // the tile's query rows, scaled row by row: D / 8 lanes a row, 16-byte units in memory's order, swizzled
       // (a row past the sequence: zeros)
-      for (int u = r; u < kRows * (D / 8); u += 128) {
-        const int rr = u / (D / 8), k = u % (D / 8);
-        const int tk = rr / p.G, hh = rr - tk * p.G;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (tk < p.tt && tok0 + tk < it.rows)
-          v = *reinterpret_cast<const uint4*>(p.q + (int64_t)(it.row0 + tok0 + tk) * p.q_stride +
-                                              (int64_t)(it.head * p.G + hh) * D + 8 * k);
-        float f[8];
-        unpack8(v, f);
-        float mx = 0.f;
+      constexpr int U = D / 8;  // units of a row, and passes over the tile
+#pragma unroll 1
+      for (int i0 = 0; i0 < U; i0 += 8) {
+        uint4 qv[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(f[i]));
-#pragma unroll
-        for (int o = 1; o < D / 8; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        const int e = pre_exponent(__float_as_uint(mx));
-        const float w = pre_pow2(kTop - e);
-        uint32_t h[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const __half2 x = __floats2half2_rn(f[2 * i] * w, f[2 * i + 1] * w);
-          h[i] = *reinterpret_cast<const uint32_t*>(&x);
+        for (int i = 0; i < 8; i++) {
+          const int rr = r / U + (128 / U) * (i0 + i);
+          const int tk = (rr * inv_g) >> 16, hh = rr - tk * p.G;
+          qv[i] = make_uint4(0, 0, 0, 0);
+          if (tk < p.tt && tok0 + tk < it.rows)
+            qv[i] = *reinterpret_cast<const uint4*>(p.q + (int64_t)(it.row0 + tok0 + tk) * p.q_stride +
+                                                    (it.head * p.G + hh) * D + 8 * (r % U));
         }
-        *reinterpret_cast<uint4*>(q_s + t * C::kTile + (k >> 3) * C::kChunk + rr * 128 + (((k & 7) ^ (rr & 7)) << 4)) =
-            make_uint4(h[0], h[1], h[2], h[3]);
-        if (k == 0) s_qexp[t][rr] = e;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const int rr = r / U + (128 / U) * (i0 + i), k = r % U;
+          float f[8];
+          unpack8(qv[i], f);
+          float mx = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(f[e]));
+#pragma unroll
+          for (int o = 1; o < U; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+          const int e = pre_exponent(__float_as_uint(mx));
+          const float w = pre_pow2(kTop - e);
+          uint32_t h[4];
+#pragma unroll
+          for (int x = 0; x < 4; x++) {
+            const __half2 y = __floats2half2_rn(f[2 * x] * w, f[2 * x + 1] * w);
+            h[x] = *reinterpret_cast<const uint32_t*>(&y);
+          }
+          *reinterpret_cast<uint4*>(q_s + t * C::kTile + (k >> 3) * C::kChunk + rr * 128 + (((k & 7) ^ (rr & 7)) << 4)) =
+              make_uint4(h[0], h[1], h[2], h[3]);
+          if (k == 0) s_qexp[t][rr] = e;
+        }
       }
       ptx::fence_proxy_async();
       ptx::mbar_arrive(&q_full[t]);
       ptx::named_bar(2 + t, 128);
       const float cq = p.scale_log2 * pre_pow2(s_qexp[t][r] - kTop);
+      more = find_item(p, BS, item_of(round), nxt);  // while the first tile is on its way
 
       // the running maximum in the log2 domain, the sum, and the exponent that O's values of V stand under
       float m = -INFINITY, l = 0.f;
@@ -452,11 +498,29 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
           for (int i = 0; i < 128; i++)
             if (key0 + i > pos) v[i] = 0xFF800000u;  // -infinity
         }
-        float mx[4];
+        // P times 2^(kPreBits + ve - vrun), back over the columns of S; the row's sum and the tile's maximum
+        float sum[4], mx[4];
+        auto soft = [&](float add) {
+          const float mc = (m == -INFINITY ? 0.f : -m) + add;
 #pragma unroll
-        for (int q = 0; q < 4; q++) mx[q] = __uint_as_float(v[q]);
+          for (int q = 0; q < 4; q++) sum[q] = 0.f, mx[q] = -INFINITY;
 #pragma unroll
-        for (int i = 4; i < 128; i++) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(v[i]));
+          for (int q = 0; q < 4; q++) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+              const float x = __uint_as_float(v[q * 32 + 2 * i]), y = __uint_as_float(v[q * 32 + 2 * i + 1]);
+              const float a = ex2(fmaf(x, c, mc)), b = ex2(fmaf(y, c, mc));
+              mx[i & 3] = fmaxf(fmaxf(mx[i & 3], x), y);
+              sum[i & 3] += a + b;
+              const __half2 h = __floats2half2_rn(a, b);
+              pk[i] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+            ptx::tmem_st16(s_t + q * 16, pk);
+          }
+        };
+        // against the maximum so far, which holds for all but a few tiles: the tile's own is known in passing
+        soft(kPreBits + (float)(ve - vrun));
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
         if (__any_sync(0xffffffffu, top > m + kPreSlack || ve > vrun)) {
           const float mn = fmaxf(m, top);
@@ -467,34 +531,19 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
           if (j > j0) {
             const float f = a * pre_pow2(max(-126, vrun - vn));
 #pragma unroll
-            for (int q = 0; q < D / 32; q++) {
-              uint32_t o[32];
-              ptx::tmem_ld32(o_t + q * 32, o);
+            for (int q = 0; q < D / 16; q++) {
+              uint32_t o[16];
+              ptx::tmem_ld16u(o_t + q * 16, o);
               ptx::tmem_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-              ptx::tmem_st32(o_t + q * 32, o);
+              for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              ptx::tmem_st16(o_t + q * 16, o);
             }
           }
           vrun = vn;
+          soft(kPreBits + (float)(ve - vrun));
         }
-        // P times 2^(kPreBits + ve - vrun)
         const float add = kPreBits + (float)(ve - vrun);
-        const float mc = (m == -INFINITY ? 0.f : -m) + add;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int q = 0; q < 4; q++) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int i = 0; i < 16; i++) {
-            const float a = ex2(fmaf(__uint_as_float(v[q * 32 + 2 * i]), c, mc));
-            const float b = ex2(fmaf(__uint_as_float(v[q * 32 + 2 * i + 1]), c, mc));
-            sum[i & 3] += a + b;
-            const __half2 h = __floats2half2_rn(a, b);
-            pk[i] = *reinterpret_cast<const uint32_t*>(&h);
-          }
-          ptx::tmem_st16(s_t + q * 16, pk);  // P over the columns of S already read
-        }
         ptx::tmem_wait_st();
         ptx::tc_fence_before();
         ptx::mbar_arrive(&p_full[t]);
