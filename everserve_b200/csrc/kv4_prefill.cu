@@ -13,7 +13,8 @@
 // A CTA keeps to its SM and walks work items: 256 rows (two tiles of 128) of one sequence and kv head,
 // over a run of 128-key tiles. Its warps:
 //   * 8-11 turn tile j's codes (loaded a tile ahead, straight to registers) into K and V stages in shared
-//     memory, 128-byte swizzled;
+//     memory, 128-byte swizzled, each freed by itself: K's by the second S, so that the next keys are there
+//     while this tile's softmax runs (one barrier for both: 711 us for the 8192-row prompt);
 //   * 12 issues the MMAs: S_t = Q_t . K_j^T and O_t += P_t . V_j for t = 0, 1 in turn, P read from TMEM;
 //   * 0-3 and 4-7 do the softmax of tiles 0 and 1, a thread a row: S from TMEM, P back over it in f16.
 // While one tile's softmax runs, the tensor core works for the other. The running maximum moves (and O in
@@ -190,28 +191,34 @@ ES_DEVICE int block_of(const PreParams& p, const Item& it, int j, int i, int tid
   return key < it.ctx ? p.block_tables[(int64_t)it.seq * p.bt_stride + key / BS] : 0;
 }
 
-// The i-th piece of key tile j, of block blk.
+// The i-th piece of key tile j, of block blk; sides: 1: K, 2: V, 3: both.
 template <int D, int NG, int BS>
-ES_DEVICE void load_raw(Raw<D, NG>& r, int i, const PreParams& p, const Item& it, int j, int tid, int64_t blk) {
+ES_DEVICE void load_raw(Raw<D, NG>& r, int i, int sides, const PreParams& p, const Item& it, int j, int tid, int64_t blk) {
   using R = Rec<D, NG, BS>;
   constexpr int P = D / 32;
   const int key = j * kKeys + i * (kConvThreads / P) + tid / P;
-  r.k[i] = r.v[i] = make_uint4(0, 0, 0, 0);  // past the history: values of zero, whatever the slot holds
+  const bool in = key < it.ctx;
+  if (in && (blk < 0 || blk >= p.num_blocks)) {  // not a block of this cache: reported, block 0 read instead
+    if (p.status) atomicExch(p.status, (int)kBadShape);
+    blk = 0;
+  }
+  const int off = key % BS;
+  const uint8_t* rec = p.cache + blk * p.s_block + (int64_t)it.head * R::kBytes;
+  // past the history: values of zero, whatever the slot holds
 #pragma unroll
-  for (int g = 0; g < NG; g++) r.km[i][g] = r.vm[i][g] = 0;
-  if (key < it.ctx) {
-    if (blk < 0 || blk >= p.num_blocks) {  // not a block of this cache: reported, block 0 read instead
-      if (p.status) atomicExch(p.status, (int)kBadShape);
-      blk = 0;
+  for (int side = 0; side < 2; side++) {
+    if (!(sides >> side & 1)) continue;
+    uint4& codes = side ? r.v[i] : r.k[i];
+    uint32_t* meta = side ? r.vm[i] : r.km[i];
+    codes = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int g = 0; g < NG; g++) meta[g] = 0;
+    if (in) {
+      codes = *reinterpret_cast<const uint4*>(rec + side * R::kV + off * R::kRow + 16 * (tid % P));
+      const uint32_t* m = reinterpret_cast<const uint32_t*>(rec + R::kKMeta + side * BS * R::kMeta + off * R::kMeta);
+#pragma unroll
+      for (int g = 0; g < NG; g++) meta[g] = m[g];
     }
-    const uint8_t* rec = p.cache + blk * p.s_block + (int64_t)it.head * R::kBytes;
-    const int off = key % BS;
-    r.k[i] = *reinterpret_cast<const uint4*>(rec + off * R::kRow + 16 * (tid % P));
-    r.v[i] = *reinterpret_cast<const uint4*>(rec + R::kV + off * R::kRow + 16 * (tid % P));
-    const uint32_t* km = reinterpret_cast<const uint32_t*>(rec + R::kKMeta + off * R::kMeta);
-    const uint32_t* vm = reinterpret_cast<const uint32_t*>(rec + R::kVMeta + off * R::kMeta);
-#pragma unroll
-    for (int g = 0; g < NG; g++) r.km[i][g] = km[g], r.vm[i][g] = vm[g];
   }
 }
 
@@ -249,12 +256,13 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
   uint8_t* q_s = smem;                  // [2] tiles
   uint8_t* kv_s = smem + 2 * C::kTile;  // [2] stages of K tile, V tile
   uint64_t* bar = reinterpret_cast<uint64_t*>(kv_s + 4 * C::kTile);
-  uint64_t *q_full = bar, *s_full = bar + 2, *p_full = bar + 4, *o_full = bar + 6, *kv_full = bar + 8, *kv_empty = bar + 10;
-  uint64_t* mma_done = bar + 12;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 13);
+  uint64_t *q_full = bar, *s_full = bar + 2, *p_full = bar + 4, *o_full = bar + 6;
+  uint64_t *k_full = bar + 8, *k_empty = bar + 10, *v_full = bar + 12, *v_empty = bar + 14;
+  uint64_t* mma_done = bar + 16;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 17);
   __shared__ int s_fail;
   __shared__ uint32_t s_bound[2][2][4];  // [tile parity][K, V][converting warp]: largest magnitudes' bits
-  __shared__ int s_exp[2][2];            // [stage][K, V]: the tile's exponents
+  __shared__ int s_exp[4][2];            // [tile & 3][K, V]: the tile's exponents
   __shared__ int s_qexp[2][kRows];       // [tile][row]: the query rows' exponents
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -265,8 +273,10 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
       ptx::mbar_init(&s_full[i], 1);
       ptx::mbar_init(&p_full[i], 128);
       ptx::mbar_init(&o_full[i], 1);
-      ptx::mbar_init(&kv_full[i], kConvThreads);
-      ptx::mbar_init(&kv_empty[i], 1);
+      ptx::mbar_init(&k_full[i], kConvThreads);
+      ptx::mbar_init(&k_empty[i], 1);
+      ptx::mbar_init(&v_full[i], kConvThreads);
+      ptx::mbar_init(&v_empty[i], 1);
     }
     ptx::mbar_init(mma_done, 1);
     ptx::fence_mbar_init();
@@ -288,7 +298,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
     constexpr int P = D / 32;
     const int tid = threadIdx.x - kSoftThreads;
     uint32_t n = 0;  // key tiles converted so far, over all items
-    for (int round = 0; ok && find_item(p, BS, item_of(round), it); round++) {
+    bool left = false;
+    for (int round = 0; !left && find_item(p, BS, item_of(round), it); round++) {
       span(p, it, j0, j1, ns);
       if (j0 >= j1) continue;
       Raw<D, NG> r;
@@ -298,7 +309,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
       for (int i = 0; i < P; i++) blk[i] = block_of<D, BS>(p, it, j0, i, tid);
 #pragma unroll
       for (int i = 0; i < P; i++) {
-        load_raw<D, NG, BS>(r, i, p, it, j0, tid, blk[i]);
+        load_raw<D, NG, BS>(r, i, 3, p, it, j0, tid, blk[i]);
         blk[i] = block_of<D, BS>(p, it, j0 + 1, i, tid);
       }
       for (int j = j0; j < j1; j++, n++) {
@@ -311,31 +322,35 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
         kb = __reduce_max_sync(0xffffffffu, kb);
         vb = __reduce_max_sync(0xffffffffu, vb);
         if (lane == 0) s_bound[s][0][warp - 8] = kb, s_bound[s][1][warp - 8] = vb;
-        if (n >= 2) ok = __all_sync(0xffffffffu, ptx::mbar_wait(&kv_empty[s], ((n >> 1) - 1) & 1));
-        if (ptx::named_bar_or(1, kConvThreads, !ok)) {  // the converting warps leave together
-          ok = false;
-          break;
-        }
+        if (n >= 2) ok = __all_sync(0xffffffffu, ptx::mbar_wait(&k_empty[s], ((n >> 1) - 1) & 1)) && ok;
+        left = ptx::named_bar_or(1, kConvThreads, !ok);  // the converting warps leave together, here alone
+        if (left) break;
         const uint32_t *bk = s_bound[s][0], *bv = s_bound[s][1];
         const int ke = pre_exponent(max(max(bk[0], bk[1]), max(bk[2], bk[3])));
         // (not far below the largest: a tile of small values leaves its probabilities' range alone)
         const int ve = max(pre_exponent(max(max(bv[0], bv[1]), max(bv[2], bv[3]))), vr - 20);
         vr = max(vr, ve);
-        if (tid == 0) s_exp[s][0] = ke, s_exp[s][1] = ve;
+        if (tid == 0) s_exp[n & 3][0] = ke, s_exp[n & 3][1] = ve;
         const float kf = pre_pow2(kTop - ke), vf = pre_pow2(kTop - ve);
         uint8_t* kt = kv_s + s * 2 * C::kTile;
 #pragma unroll
         for (int i = 0; i < P; i++) {
-          const int row = i * (kConvThreads / P) + tid / P;
-          store_piece<D, NG>(kt, row, tid % P, r.k[i], r.km[i], kf);
-          store_piece<D, NG>(kt + C::kTile, row, tid % P, r.v[i], r.vm[i], vf);
+          store_piece<D, NG>(kt, i * (kConvThreads / P) + tid / P, tid % P, r.k[i], r.km[i], kf);
+          if (j + 1 < j1) load_raw<D, NG, BS>(r, i, 1, p, it, j + 1, tid, blk[i]);
+        }
+        ptx::fence_proxy_async();
+        ptx::mbar_arrive(&k_full[s]);
+        if (n >= 2) ok = __all_sync(0xffffffffu, ptx::mbar_wait(&v_empty[s], ((n >> 1) - 1) & 1));
+#pragma unroll
+        for (int i = 0; i < P; i++) {
+          store_piece<D, NG>(kt + C::kTile, i * (kConvThreads / P) + tid / P, tid % P, r.v[i], r.vm[i], vf);
           if (j + 1 < j1) {
-            load_raw<D, NG, BS>(r, i, p, it, j + 1, tid, blk[i]);
+            load_raw<D, NG, BS>(r, i, 2, p, it, j + 1, tid, blk[i]);
             blk[i] = block_of<D, BS>(p, it, j + 2, i, tid);
           }
         }
         ptx::fence_proxy_async();
-        ptx::mbar_arrive(&kv_full[s]);
+        ptx::mbar_arrive(&v_full[s]);
       }
     }
     if (!ok) s_fail = 1;
@@ -361,13 +376,14 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
           ptx::mma_f16_ss(tmem + t * 128, a + off, b + off, idesc_s, kk > 0 ? 1u : 0u);
         }
         ptx::mma_commit(&s_full[t]);
+        if (t == 1) ptx::mma_commit(&k_empty[s]);
       }
       __syncwarp();
     };
     for (int round = 0; ok && find_item(p, BS, item_of(round), it); round++) {
       span(p, it, j0, j1, ns);
       if (j0 >= j1) continue;
-      ok = __all_sync(0xffffffffu, ptx::mbar_wait(&kv_full[n & 1], (n >> 1) & 1));
+      ok = __all_sync(0xffffffffu, ptx::mbar_wait(&k_full[n & 1], (n >> 1) & 1));
       for (int t = 0; ok && t < 2; t++) {
         ok = __all_sync(0xffffffffu, ptx::mbar_wait(&q_full[t], items & 1));
         if (!ok) break;
@@ -378,6 +394,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
         const int s = n & 1;
 #pragma unroll
         for (int t = 0; t < 2; t++) {
+          if (t == 0) ok = __all_sync(0xffffffffu, ptx::mbar_wait(&v_full[s], (n >> 1) & 1));
           ok = ok && __all_sync(0xffffffffu, ptx::mbar_wait(&p_full[t], n & 1));
           if (!ok) break;
           ptx::tc_fence_after();
@@ -387,12 +404,12 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
             for (int kk = 0; kk < kKeys / 16; kk++)
               ptx::mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, b + kk * (16 * 128 >> 4), idesc_o,
                               (j > j0 || kk > 0) ? 1u : 0u);
-            if (t == 1) ptx::mma_commit(&kv_empty[s]);
+            if (t == 1) ptx::mma_commit(&v_empty[s]);
             if (j + 1 == j1) ptx::mma_commit(&o_full[t]);
           }
           __syncwarp();
           if (j + 1 < j1) {
-            if (t == 0) ok = __all_sync(0xffffffffu, ptx::mbar_wait(&kv_full[s ^ 1], ((n + 1) >> 1) & 1));
+            if (t == 0) ok = __all_sync(0xffffffffu, ptx::mbar_wait(&k_full[s ^ 1], ((n + 1) >> 1) & 1));
             if (!ok) break;
             ptx::tc_fence_after();
             qk(t, s ^ 1);  // after P_t . V in the tensor core's order, which P_t's columns wait for
@@ -486,8 +503,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
         ok = __all_sync(0xffffffffu, ptx::mbar_wait(&s_full[t], n & 1));
         if (!ok) break;
         ptx::tc_fence_after();
-        const float c = cq * pre_pow2(s_exp[n & 1][0] - kTop);
-        const int ve = s_exp[n & 1][1];
+        const float c = cq * pre_pow2(s_exp[n & 3][0] - kTop);
+        const int ve = s_exp[n & 3][1];
         uint32_t v[128];
 #pragma unroll
         for (int q = 0; q < 4; q++) ptx::tmem_ld32(s_t + q * 32, v + q * 32);
