@@ -301,6 +301,7 @@ struct Kv4PrefillArgs {
   float* part_o;   // [T, hq, max_splits, d] (unused with one split)
   float* part_ml;  // [T, hq, max_splits, 2]
   int* part_ns;    // [T]
+  unsigned* next;  // a word the launch zeroes
   int* status;
   int64_t T, S;
   int hq, max_splits, num_sms;

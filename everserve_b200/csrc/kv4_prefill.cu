@@ -23,8 +23,8 @@
 //
 // A sequence with few rows and a long history is cut along its keys as well, into items whose results
 // (O, m, l) a second kernel joins. The cut depends on the sequence's own rows and keys and on the model's
-// heads, never on the batch. Each warp finds its item by a scan over the sequences, so the host needs no
-// plan and no synchronisation. All waits are bounded and end in the status word.
+// heads, never on the batch. An item is found by a scan over the sequences, so the host needs no
+// plan and no synchronisation; a warp of each CTA hands out items ahead of their readers. All waits are bounded and end in the status word.
 #include <atomic>
 
 #include "api.h"
@@ -77,6 +77,7 @@ struct PreParams {
   float* part_ml;      // [T, hq, max_splits, 2]
   int* part_ns;        // [T]
   int* status;
+  unsigned* next;      // items handed out beyond each CTA's first, zero before the launch
   int T, S, hq, hkv, G, tt, max_splits;  // tt: tokens of a 128-row tile
   float scale_log2;
 };
@@ -91,10 +92,11 @@ __host__ __device__ __forceinline__ int chunk_of(int tiles, int hkv) {
 struct Item {
   int seq, rows, row0, ctx;  // the sequence, its rows, its first row, its context length
   int tile, head, split, chunk;
+  int j0, j1, ns;  // its key tiles, and how many items its row tile has
 };
 
-// Work item `idx`, in an order that starts with a sequence's last (longest) tiles; false: there is none.
-// The whole warp calls it.
+// Work item `idx`, in an order that puts long ones first: of 32 sequences at a time those with the most keys,
+// of a sequence its last tiles. False: there is none. The whole warp calls it.
 ES_DEVICE bool find_item(const PreParams& p, int bs, int idx, Item& it) {
   const int lane = threadIdx.x & 31;
   int before = 0;
@@ -111,6 +113,20 @@ ES_DEVICE bool find_item(const PreParams& p, int bs, int idx, Item& it) {
       ns = max(1, min(p.max_splits, ((ctx + kKeys - 1) / kKeys + chunk - 1) / chunk));
       items = tiles * ns * p.hkv;
     }
+    // this lane's place in the order: the sequence (lane) `src`
+    int src = lane;
+    if (p.S > 1) {
+      int rank = 0;
+#pragma unroll 4
+      for (int k = 0; k < 32; k++) {
+        const int c = __shfl_sync(0xffffffffu, ctx, k);
+        rank += c > ctx || (c == ctx && k < lane);
+      }
+#pragma unroll 4
+      for (int k = 0; k < 32; k++)
+        if (__shfl_sync(0xffffffffu, rank, k) == lane) src = k;
+      items = __shfl_sync(0xffffffffu, items, src);
+    }
     int upto = items;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -119,8 +135,9 @@ ES_DEVICE bool find_item(const PreParams& p, int bs, int idx, Item& it) {
     }
     const int total = __shfl_sync(0xffffffffu, upto, 31);
     if (idx < before + total) {
-      const int src = __ffs(__ballot_sync(0xffffffffu, idx < before + upto)) - 1;
-      const int first = before + __shfl_sync(0xffffffffu, upto - items, src);
+      const int place = __ffs(__ballot_sync(0xffffffffu, idx < before + upto)) - 1;
+      const int first = before + __shfl_sync(0xffffffffu, upto - items, place);
+      src = __shfl_sync(0xffffffffu, src, place);
       it.seq = s0 + src;
       it.rows = __shfl_sync(0xffffffffu, rows, src);
       it.row0 = __shfl_sync(0xffffffffu, r0, src);
@@ -138,20 +155,15 @@ ES_DEVICE bool find_item(const PreParams& p, int bs, int idx, Item& it) {
   return false;
 }
 
-// A CTA's item of a round: every other round the other way, as an item's length falls along the order.
-ES_DEVICE int item_of(int round) {
-  return round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-}
-
-// The key tiles [j0, j1) of an item, and how many items its row tile has.
-ES_DEVICE void span(const PreParams& p, const Item& it, int& j0, int& j1, int& ns) {
+// The key tiles of an item, and how many items its row tile has.
+ES_DEVICE void span(const PreParams& p, Item& it) {
   const int last = min(it.rows, (it.tile + 1) * 2 * p.tt) - 1;  // the tile's last token
   const int pos = min(it.ctx - it.rows + last, it.ctx - 1);
   const int J = pos < 0 ? 0 : pos / kKeys + 1;
-  ns = max(1, min(p.max_splits, (J - 1) / it.chunk + 1));
-  j0 = it.split * it.chunk;
-  j1 = it.split == ns - 1 ? J : min(J, j0 + it.chunk);
-  if (it.split >= ns) j1 = j0;
+  it.ns = max(1, min(p.max_splits, (J - 1) / it.chunk + 1));
+  it.j0 = it.split * it.chunk;
+  it.j1 = it.split == it.ns - 1 ? J : min(J, it.j0 + it.chunk);
+  if (it.split >= it.ns) it.j1 = it.j0;
 }
 
 // 8 codes -> 8 f16 values: a masked nibble under the exponent of 1024 (bits 0..3) or 64 (bits 4..7) is
@@ -175,52 +187,46 @@ ES_DEVICE uint4 values8(uint32_t w, __half2 s, __half2 z) {
 ES_DEVICE float pre_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 ES_DEVICE int pre_exponent(uint32_t bits) { return min(100, max(-40, (int)(bits >> 23) - 127)); }
 
-// What a converting thread holds of a key tile: 16-byte pieces (32 codes) of K and of V rows.
-template <int D, int NG>
-struct Raw {
-  static constexpr int kPer = D / 32;  // pieces of a row, and passes over the 128 rows
-  uint4 k[kPer], v[kPer];
-  uint32_t km[kPer][NG], vm[kPer][NG];
-};
-
-// The block of the key that a thread's i-th piece of key tile j belongs to (0 past the history).
-template <int D, int BS>
-ES_DEVICE int block_of(const PreParams& p, const Item& it, int j, int i, int tid) {
-  constexpr int P = D / 32;
-  const int key = j * kKeys + i * (kConvThreads / P) + tid / P;
-  return key < it.ctx ? p.block_tables[(int64_t)it.seq * p.bt_stride + key / BS] : 0;
-}
-
-// The i-th piece of key tile j, of block blk; sides: 1: K, 2: V, 3: both.
+// Where a converting thread reads: row tid / P of each pass of kConvThreads / P rows, piece tid % P of the
+// row. A pass is a multiple of a block, so a thread stays at one row of its blocks.
 template <int D, int NG, int BS>
-ES_DEVICE void load_raw(Raw<D, NG>& r, int i, int sides, const PreParams& p, const Item& it, int j, int tid, int64_t blk) {
+struct Source {
   using R = Rec<D, NG, BS>;
-  constexpr int P = D / 32;
-  const int key = j * kKeys + i * (kConvThreads / P) + tid / P;
-  const bool in = key < it.ctx;
-  if (in && (blk < 0 || blk >= p.num_blocks)) {  // not a block of this cache: reported, block 0 read instead
-    if (p.status) atomicExch(p.status, (int)kBadShape);
-    blk = 0;
-  }
-  const int off = key % BS;
-  const uint8_t* rec = p.cache + blk * p.s_block + (int64_t)it.head * R::kBytes;
-  // past the history: values of zero, whatever the slot holds
-#pragma unroll
-  for (int side = 0; side < 2; side++) {
-    if (!(sides >> side & 1)) continue;
-    uint4& codes = side ? r.v[i] : r.k[i];
-    uint32_t* meta = side ? r.vm[i] : r.km[i];
+  static constexpr int P = D / 32;
+  const int* bt;        // the sequence's table, from this thread's first block of tile 0
+  const uint8_t* base;  // this thread's piece of its row, in block 0
+  uint32_t step;        // 16-byte units between blocks
+  int first, ctx, piece;
+  int64_t num_blocks;
+  bool bad = false;  // met an entry that is not a block of this cache
+
+  ES_DEVICE Source(const PreParams& p, const Item& it, int tid)
+      : bt(p.block_tables + (int64_t)it.seq * p.bt_stride),
+        base(p.cache + (int64_t)it.head * R::kBytes + tid / P % BS * R::kRow),
+        step((uint32_t)(p.s_block >> 4)),
+        first(tid / P),
+        ctx(it.ctx),
+        piece(tid % P),
+        num_blocks(p.num_blocks) {}
+  ES_DEVICE int key(int j, int i) const { return j * kKeys + i * (kConvThreads / P) + first; }
+  ES_DEVICE int block(int j, int i) const { return key(j, i) < ctx ? bt[key(j, i) / BS] : 0; }
+  // The codes and pairs of the i-th piece of tile j, side 0: K, 1: V (zero past the history, whatever the
+  // slot holds: its values are zero then).
+  ES_DEVICE void load(int j, int i, int blk, int side, uint4& codes, uint32_t* meta) {
     codes = make_uint4(0, 0, 0, 0);
 #pragma unroll
     for (int g = 0; g < NG; g++) meta[g] = 0;
-    if (in) {
-      codes = *reinterpret_cast<const uint4*>(rec + side * R::kV + off * R::kRow + 16 * (tid % P));
-      const uint32_t* m = reinterpret_cast<const uint32_t*>(rec + R::kKMeta + side * BS * R::kMeta + off * R::kMeta);
+    if (key(j, i) < ctx) {
+      if ((uint32_t)blk >= (uint64_t)num_blocks) bad = true, blk = 0;
+      const uint8_t* row = base + ((uint64_t)(uint32_t)blk * step << 4);
+      codes = *reinterpret_cast<const uint4*>(row + side * R::kV + 16 * piece);
+      const int off = first % BS;
+      const uint32_t* m = reinterpret_cast<const uint32_t*>(row + R::kKMeta + side * BS * R::kMeta + off * (R::kMeta - R::kRow));
 #pragma unroll
       for (int g = 0; g < NG; g++) meta[g] = m[g];
     }
   }
-}
+};
 
 // The bits of a bound on a group's magnitudes.
 ES_DEVICE uint32_t bound_of(uint32_t pair) {
@@ -259,16 +265,19 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
   uint64_t *q_full = bar, *s_full = bar + 2, *p_full = bar + 4, *o_full = bar + 6;
   uint64_t *k_full = bar + 8, *k_empty = bar + 10, *v_full = bar + 12, *v_empty = bar + 14;
   uint64_t* mma_done = bar + 16;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 17);
+  uint64_t *item_full = bar + 17, *item_empty = bar + 19;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 21);
   __shared__ int s_fail;
+  __shared__ Item s_item[2];             // items ahead of their readers; seq -1: there is none
   __shared__ uint32_t s_bound[2][2][4];  // [tile parity][K, V][converting warp]: largest magnitudes' bits
   __shared__ int s_exp[4][2];            // [tile & 3][K, V]: the tile's exponents
-  __shared__ int s_qexp[2][kRows];       // [tile][row]: the query rows' exponents
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     s_fail = 0;
     for (int i = 0; i < 2; i++) {
+      ptx::mbar_init(&item_full[i], 1);
+      ptx::mbar_init(&item_empty[i], 13);  // a lane of every warp that reads items
       ptx::mbar_init(&q_full[i], 128);
       ptx::mbar_init(&s_full[i], 1);
       ptx::mbar_init(&p_full[i], 128);
@@ -290,8 +299,19 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
   pdl_launch();
 
   Item it;
-  int j0, j1, ns;
   bool ok = true;
+  // The warp's next item, in order, into `it` (false: none, or a wait ran out).
+  uint32_t taken = 0;
+  auto next_item = [&]() {
+    const int s = taken & 1;
+    ok = __all_sync(0xffffffffu, ptx::mbar_wait(&item_full[s], (taken >> 1) & 1));
+    if (!ok) return false;
+    it = s_item[s];
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(&item_empty[s]);
+    taken++;
+    return it.seq >= 0;
+  };
   if (warp >= 8 && warp < 12) {
     // ---- codes to values ------------------------------------------------------------------------
     regs_down<kConvRegs>();
@@ -299,31 +319,39 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
     const int tid = threadIdx.x - kSoftThreads;
     uint32_t n = 0;  // key tiles converted so far, over all items
     bool left = false;
-    for (int round = 0; !left && find_item(p, BS, item_of(round), it); round++) {
-      span(p, it, j0, j1, ns);
-      if (j0 >= j1) continue;
-      Raw<D, NG> r;
+    while (!left) {
+      const bool any = next_item();
+      left = ptx::named_bar_or(1, kConvThreads, !ok);  // where a wait of one of the converting warps ran out, all leave
+      if (left || !any) break;
+      if (it.j0 >= it.j1) continue;
+      Source<D, NG, BS> src(p, it, tid);
+      uint4 kc[P], vc[P];  // the next tile's codes and pairs
+      uint32_t km[P][NG], vm[P][NG];
+      int blk[P];  // and its blocks: a table entry is asked for two tiles ahead, its data one
       int vr = -100;  // the largest of V's exponents so far
-      int blk[P];     // the next tile's blocks: a table entry is asked for two tiles ahead, its data one
 #pragma unroll
-      for (int i = 0; i < P; i++) blk[i] = block_of<D, BS>(p, it, j0, i, tid);
+      for (int i = 0; i < P; i++) blk[i] = src.block(it.j0, i);
 #pragma unroll
       for (int i = 0; i < P; i++) {
-        load_raw<D, NG, BS>(r, i, 3, p, it, j0, tid, blk[i]);
-        blk[i] = block_of<D, BS>(p, it, j0 + 1, i, tid);
+        src.load(it.j0, i, blk[i], 0, kc[i], km[i]);
+        src.load(it.j0, i, blk[i], 1, vc[i], vm[i]);
+        blk[i] = src.block(it.j0 + 1, i);
       }
-      for (int j = j0; j < j1; j++, n++) {
+#pragma unroll 1
+      for (int j = it.j0; j < it.j1; j++, n++) {
         const int s = n & 1;
+        uint8_t* kt = kv_s + s * 2 * C::kTile;
+        // the tile's largest magnitudes over the converting warps, whose barrier is where they leave together
         uint32_t kb = 0, vb = 0;
 #pragma unroll
         for (int i = 0; i < P; i++)
 #pragma unroll
-          for (int g = 0; g < NG; g++) kb = max(kb, bound_of(r.km[i][g])), vb = max(vb, bound_of(r.vm[i][g]));
+          for (int g = 0; g < NG; g++) kb = max(kb, bound_of(km[i][g])), vb = max(vb, bound_of(vm[i][g]));
         kb = __reduce_max_sync(0xffffffffu, kb);
         vb = __reduce_max_sync(0xffffffffu, vb);
         if (lane == 0) s_bound[s][0][warp - 8] = kb, s_bound[s][1][warp - 8] = vb;
         if (n >= 2) ok = __all_sync(0xffffffffu, ptx::mbar_wait(&k_empty[s], ((n >> 1) - 1) & 1)) && ok;
-        left = ptx::named_bar_or(1, kConvThreads, !ok);  // the converting warps leave together, here alone
+        left = ptx::named_bar_or(1, kConvThreads, !ok);
         if (left) break;
         const uint32_t *bk = s_bound[s][0], *bv = s_bound[s][1];
         const int ke = pre_exponent(max(max(bk[0], bk[1]), max(bk[2], bk[3])));
@@ -332,31 +360,52 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
         vr = max(vr, ve);
         if (tid == 0) s_exp[n & 3][0] = ke, s_exp[n & 3][1] = ve;
         const float kf = pre_pow2(kTop - ke), vf = pre_pow2(kTop - ve);
-        uint8_t* kt = kv_s + s * 2 * C::kTile;
+        const bool on = j + 1 < it.j1;
 #pragma unroll
         for (int i = 0; i < P; i++) {
-          store_piece<D, NG>(kt, i * (kConvThreads / P) + tid / P, tid % P, r.k[i], r.km[i], kf);
-          if (j + 1 < j1) load_raw<D, NG, BS>(r, i, 1, p, it, j + 1, tid, blk[i]);
+          store_piece<D, NG>(kt, i * (kConvThreads / P) + tid / P, tid % P, kc[i], km[i], kf);
+          if (on) src.load(j + 1, i, blk[i], 0, kc[i], km[i]);
         }
         ptx::fence_proxy_async();
         ptx::mbar_arrive(&k_full[s]);
         if (n >= 2) ok = __all_sync(0xffffffffu, ptx::mbar_wait(&v_empty[s], ((n >> 1) - 1) & 1));
 #pragma unroll
         for (int i = 0; i < P; i++) {
-          store_piece<D, NG>(kt + C::kTile, i * (kConvThreads / P) + tid / P, tid % P, r.v[i], r.vm[i], vf);
-          if (j + 1 < j1) {
-            load_raw<D, NG, BS>(r, i, 2, p, it, j + 1, tid, blk[i]);
-            blk[i] = block_of<D, BS>(p, it, j + 2, i, tid);
+          store_piece<D, NG>(kt + C::kTile, i * (kConvThreads / P) + tid / P, tid % P, vc[i], vm[i], vf);
+          if (on) {
+            src.load(j + 1, i, blk[i], 1, vc[i], vm[i]);
+            blk[i] = src.block(j + 2, i);
           }
         }
         ptx::fence_proxy_async();
         ptx::mbar_arrive(&v_full[s]);
       }
+      if (src.bad && p.status) atomicExch(p.status, (int)kBadShape);
     }
     if (!ok) s_fail = 1;
   } else if (warp >= 12) {
-    // ---- MMA issuer (the group's other warps idle) -------------------------------------------------
+    // ---- MMA issuer, and the warp that hands out items (the group's other two idle) -----------------
     regs_down<kMmaRegs>();
+    if (warp == 13) {
+      // An item's cost goes with its keys, so CTAs take their next one when they are ready for it, from one
+      // counter (in turn: up to half of them waited for the longest, 16 prompts took 172 us).
+      int idx = blockIdx.x;
+      for (uint32_t k = 0; ok; k++) {
+        const bool any = find_item(p, BS, idx, it);
+        if (any) span(p, it);
+        if (k >= 2) ok = __all_sync(0xffffffffu, ptx::mbar_wait(&item_empty[k & 1], ((k >> 1) - 1) & 1));
+        if (!ok) break;
+        if (lane == 0) {
+          if (!any) it.seq = -1;
+          s_item[k & 1] = it;
+          ptx::mbar_arrive(&item_full[k & 1]);
+        }
+        if (!any) break;
+        if (lane == 0) idx = (int)(gridDim.x + atomicAdd(p.next, 1u));
+        idx = __shfl_sync(0xffffffffu, idx, 0);
+      }
+    }
+    const bool failed = !ok;
     ok = warp == 12;
     constexpr uint32_t idesc_s = ptx::idesc_f16_f32(kRows, kKeys);
     constexpr uint32_t idesc_o = ptx::idesc_f16_f32(kRows, D) | (1u << 16);  // V: MN-major
@@ -380,8 +429,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
       }
       __syncwarp();
     };
-    for (int round = 0; ok && find_item(p, BS, item_of(round), it); round++) {
-      span(p, it, j0, j1, ns);
+    while (ok && next_item()) {
+      const int j0 = it.j0, j1 = it.j1;
       if (j0 >= j1) continue;
       ok = __all_sync(0xffffffffu, ptx::mbar_wait(&k_full[n & 1], (n >> 1) & 1));
       for (int t = 0; ok && t < 2; t++) {
@@ -418,8 +467,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
       }
       items++;
     }
+    if (failed || (warp == 12 && !ok)) s_fail = 1;
     if (warp == 12) {
-      if (!ok) s_fail = 1;
       if (leader) ptx::mma_commit(mma_done);
       __syncwarp();
       ptx::mbar_wait(mma_done, 0);  // nothing of this CTA is in flight past here
@@ -433,68 +482,73 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
     const uint32_t s_t = tmem + t * 128 + lane_base, o_t = tmem + 256 + t * 128 + lane_base;
     const int inv_g = (65536 + p.G - 1) / p.G;  // x / G = (x * inv_g) >> 16 for x < 128
     const int token = (r * inv_g) >> 16, head = r - token * p.G;
+    // This warp's 32 rows of the query tile, which no other warp touches: D / 8 lanes a row and 32 / U rows a
+    // pass where memory is read or written, a thread a row where a row is scaled. unit(): 16-byte unit k of
+    // row x in the tile's swizzled layout.
+    constexpr int U = D / 8, kPass = 32 / U;
+    const int w0 = (warp & 3) * 32;
+    uint8_t* rows_s = q_s + t * C::kTile;
+    auto unit = [&](int x, int k) {
+      return reinterpret_cast<uint4*>(rows_s + (k >> 3) * C::kChunk + x * 128 + (((k & 7) ^ (x & 7)) << 4));
+    };
+    // where row x of an item's tile is in memory (elements of q, of the output), or -1 past the sequence
+    auto row_of = [&](const Item& i, int x, int64_t stride) -> int64_t {
+      const int tk = (x * inv_g) >> 16, hh = x - tk * p.G;
+      const int at = i.tile * 2 * p.tt + t * p.tt + tk;
+      return tk < p.tt && at < i.rows ? (int64_t)(i.row0 + at) * stride + (i.head * p.G + hh) * D : -1;
+    };
     uint32_t n = 0, items = 0;
-    Item nxt;
-    bool more = find_item(p, BS, item_of(0), nxt);
-    for (int round = 1; ok && more; round++) {
-      it = nxt;
-      span(p, it, j0, j1, ns);
-      const int tok0 = it.tile * 2 * p.tt + t * p.tt;  // the tile's first token of the sequence
-      const int at = tok0 + token;
-      const bool real = token < p.tt && at < it.rows;
-      const int64_t row = it.row0 + at;
+    while (ok && next_item()) {
+      const int j0 = it.j0, j1 = it.j1, ns = it.ns;
+      const int64_t out_row = row_of(it, r, (int64_t)p.hq * D);  // -1: no row
+      const int at = it.tile * 2 * p.tt + t * p.tt + token;
       const int pos = it.ctx - it.rows + at;
-      __nv_bfloat16* out = p.out + (row * p.hq + it.head * p.G + head) * (int64_t)D;
-      if (real && it.split == 0 && it.head == 0 && head == 0 && p.part_ns != nullptr) p.part_ns[row] = ns;
+      if (out_row >= 0 && it.split == 0 && it.head == 0 && head == 0 && p.part_ns != nullptr) p.part_ns[it.row0 + at] = ns;
       if (j0 >= j1) {
-        if (it.split == 0 && real)  // no key at all
-          for (int i = 0; i < D / 8; i++) reinterpret_cast<uint4*>(out)[i] = make_uint4(0, 0, 0, 0);
-        more = find_item(p, BS, item_of(round), nxt);
+        if (it.split == 0 && out_row >= 0)  // no key at all
+          for (int i = 0; i < U; i++) reinterpret_cast<uint4*>(p.out + out_row)[i] = make_uint4(0, 0, 0, 0);
         continue;
       }
-      // the tile's query rows, scaled row by row: D / 8 lanes a row, 16-byte units in memory's order, swizzled
-      // (a row past the sequence: zeros)
-      constexpr int U = D / 8;  // units of a row, and passes over the tile
-#pragma unroll 1
-      for (int i0 = 0; i0 < U; i0 += 8) {
-        uint4 qv[8];
+      // the query: asynchronous copies in memory's order, then each thread scales its own row by a power of two
+#pragma unroll 4
+      for (int x = 0; x < U; x++) {
+        const int rr = w0 + x * kPass + lane / U;
+        const int64_t at = row_of(it, rr, p.q_stride);
+        ptx::cp_async16(unit(rr, lane % U), p.q + max(at, (int64_t)0) + 8 * (lane % U), at >= 0);
+      }
+      ptx::cp_async_wait_all();
+      __syncwarp();
+      float cq;
+      {
+        uint4 qv[U];
+        __nv_bfloat162 mx = __floats2bfloat162_rn(0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const int rr = r / U + (128 / U) * (i0 + i);
-          const int tk = (rr * inv_g) >> 16, hh = rr - tk * p.G;
-          qv[i] = make_uint4(0, 0, 0, 0);
-          if (tk < p.tt && tok0 + tk < it.rows)
-            qv[i] = *reinterpret_cast<const uint4*>(p.q + (int64_t)(it.row0 + tok0 + tk) * p.q_stride +
-                                                    (it.head * p.G + hh) * D + 8 * (r % U));
+        for (int k = 0; k < U; k++) qv[k] = *unit(r, k);
+#pragma unroll
+        for (int k = 0; k < U; k++) {
+          const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&qv[k]);
+#pragma unroll
+          for (int e = 0; e < 4; e++) mx = __hmax2(mx, __habs2(h[e]));
         }
+        const float2 m2 = __bfloat1622float2(mx);
+        const int qe = pre_exponent(__float_as_uint(fmaxf(m2.x, m2.y)));
+        const float qf = pre_pow2(kTop - qe);
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const int rr = r / U + (128 / U) * (i0 + i), k = r % U;
+        for (int k = 0; k < U; k++) {
           float f[8];
-          unpack8(qv[i], f);
-          float mx = 0.f;
-#pragma unroll
-          for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(f[e]));
-#pragma unroll
-          for (int o = 1; o < U; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-          const int e = pre_exponent(__float_as_uint(mx));
-          const float w = pre_pow2(kTop - e);
+          unpack8(qv[k], f);
           uint32_t h[4];
 #pragma unroll
           for (int x = 0; x < 4; x++) {
-            const __half2 y = __floats2half2_rn(f[2 * x] * w, f[2 * x + 1] * w);
+            const __half2 y = __floats2half2_rn(f[2 * x] * qf, f[2 * x + 1] * qf);
             h[x] = *reinterpret_cast<const uint32_t*>(&y);
           }
-          *reinterpret_cast<uint4*>(q_s + t * C::kTile + (k >> 3) * C::kChunk + rr * 128 + (((k & 7) ^ (rr & 7)) << 4)) =
-              make_uint4(h[0], h[1], h[2], h[3]);
-          if (k == 0) s_qexp[t][rr] = e;
+          *unit(r, k) = make_uint4(h[0], h[1], h[2], h[3]);
         }
+        cq = p.scale_log2 * pre_pow2(qe - kTop);
       }
       ptx::fence_proxy_async();
       ptx::mbar_arrive(&q_full[t]);
-      ptx::named_bar(2 + t, 128);
-      const float cq = p.scale_log2 * pre_pow2(s_qexp[t][r] - kTop);
-      more = find_item(p, BS, item_of(round), nxt);  // while the first tile is on its way
 
       // the running maximum in the log2 domain, the sum, and the exponent that O's values of V stand under
       float m = -INFINITY, l = 0.f;
@@ -514,6 +568,15 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
 #pragma unroll
           for (int i = 0; i < 128; i++)
             if (key0 + i > pos) v[i] = 0xFF800000u;  // -infinity
+        }
+        if (j == j0) {  // the first keys: their maximum, and nothing to rescale
+          float mx[4];
+#pragma unroll
+          for (int q = 0; q < 4; q++) mx[q] = __uint_as_float(v[q]);
+#pragma unroll
+          for (int i = 4; i < 128; i++) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(v[i]));
+          m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
+          vrun = ve;
         }
         // P times 2^(kPreBits + ve - vrun), back over the columns of S; the row's sum and the tile's maximum
         float sum[4], mx[4];
@@ -547,7 +610,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
           l *= a;
           if (j > j0) {
             const float f = a * pre_pow2(max(-126, vrun - vn));
-#pragma unroll
+#pragma unroll 1
             for (int q = 0; q < D / 16; q++) {
               uint32_t o[16];
               ptx::tmem_ld16u(o_t + q * 16, o);
@@ -570,34 +633,52 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
       if (!ok) break;
       items++;
       ptx::tc_fence_after();
-      const float unit = pre_pow2(vrun - kTop - (int)kPreBits);
-      const float inv = l > 0.f || l != l ? unit / l : 0.f;
-      const int64_t part = (row * p.hq + it.head * p.G + head) * (int64_t)p.max_splits + it.split;
+      // the output: through this warp's rows of the query tile (read by no MMA any more), so that a store
+      // covers whole rows; a split's in fp32, each thread its row
+      const float unit_o = pre_pow2(vrun - kTop - (int)kPreBits);
+      const bool none = !(l > 0.f || l != l);  // no visible key: zeros
+      const float scale_o = ns > 1 ? unit_o : none ? 0.f : unit_o / l;
+      const int64_t part = out_row / D * p.max_splits + it.split;
+      if (ns == 1) {
 #pragma unroll
-      for (int q = 0; q < D / 32; q++) {
-        uint32_t v[32];
-        ptx::tmem_ld32(o_t + q * 32, v);
-        ptx::tmem_wait_ld();
-        if (!real) continue;
-        if (ns == 1) {
+        for (int q = 0; q < D / 32; q++) {
+          uint32_t v[32];
+          ptx::tmem_ld32(o_t + q * 32, v);
+          ptx::tmem_wait_ld();
 #pragma unroll
           for (int u = 0; u < 4; u++) {
             float f[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) f[i] = l > 0.f || l != l ? __uint_as_float(v[u * 8 + i]) * inv : 0.f;
-            reinterpret_cast<uint4*>(out)[q * 4 + u] = pack8(f);
+            for (int i = 0; i < 8; i++) f[i] = none ? 0.f : __uint_as_float(v[u * 8 + i]) * scale_o;
+            *unit(r, q * 4 + u) = pack8(f);
           }
-        } else {
+        }
+        __syncwarp();
+#pragma unroll 8
+        for (int x = 0; x < U; x++) {
+          const int rr = w0 + x * kPass + lane / U;
+          const int64_t at = row_of(it, rr, (int64_t)p.hq * D);
+          const uint4 y = *unit(rr, lane % U);
+          if (at >= 0) reinterpret_cast<uint4*>(p.out + at)[lane % U] = y;
+        }
+        __syncwarp();
+      } else {
+#pragma unroll 1
+        for (int q = 0; q < D / 32; q++) {
+          uint32_t v[32];
+          ptx::tmem_ld32(o_t + q * 32, v);
+          ptx::tmem_wait_ld();
+          if (out_row < 0) continue;
 #pragma unroll
           for (int u = 0; u < 8; u++) {
             float4 f;
-            f.x = __uint_as_float(v[4 * u]) * unit, f.y = __uint_as_float(v[4 * u + 1]) * unit;
-            f.z = __uint_as_float(v[4 * u + 2]) * unit, f.w = __uint_as_float(v[4 * u + 3]) * unit;
+            f.x = __uint_as_float(v[4 * u]) * scale_o, f.y = __uint_as_float(v[4 * u + 1]) * scale_o;
+            f.z = __uint_as_float(v[4 * u + 2]) * scale_o, f.w = __uint_as_float(v[4 * u + 3]) * scale_o;
             reinterpret_cast<float4*>(p.part_o + part * D)[q * 8 + u] = f;
           }
         }
       }
-      if (real && ns > 1) p.part_ml[2 * part] = m, p.part_ml[2 * part + 1] = l;
+      if (out_row >= 0 && ns > 1) p.part_ml[2 * part] = m, p.part_ml[2 * part + 1] = l;
       ptx::tc_fence_before();
     }
     if (!ok) s_fail = 1;
@@ -666,6 +747,7 @@ cudaError_t launch_kv4_prefill(const Kv4PrefillArgs& a, cudaStream_t stream) {
   if (a.T == 0 || a.S == 0) return cudaSuccess;
   if (a.c.hkv <= 0 || a.hq % a.c.hkv != 0 || a.hq / a.c.hkv > kv4::kRows || a.max_splits < 1 || !(a.scale > 0.f))
     return cudaErrorInvalidValue;
+  if (a.c.s_block >> 4 > UINT32_MAX) return cudaErrorInvalidValue;
   if (a.T > INT32_MAX / 2 || a.bt_cols * a.c.block_size > INT32_MAX - kv4::kKeys || a.T * a.hq > ((int64_t)1 << 32))
     return cudaErrorInvalidValue;
   kv4::PreParams p{};
@@ -683,6 +765,7 @@ cudaError_t launch_kv4_prefill(const Kv4PrefillArgs& a, cudaStream_t stream) {
   p.part_o = a.part_o;
   p.part_ml = a.part_ml;
   p.part_ns = a.max_splits > 1 ? a.part_ns : nullptr;
+  p.next = a.next;
   p.status = a.status;
   p.T = (int)a.T;
   p.S = (int)a.S;
@@ -695,6 +778,8 @@ cudaError_t launch_kv4_prefill(const Kv4PrefillArgs& a, cudaStream_t stream) {
   // items: at most a row tile per 2 tt rows and sequence, each times heads and splits
   const int64_t most = (a.T / (2 * p.tt) + a.S) * p.hkv * a.max_splits;
   const int grid = (int)(most < a.num_sms ? most : a.num_sms);
+  const cudaError_t e = cudaMemsetAsync(a.next, 0, sizeof(unsigned), stream);
+  if (e != cudaSuccess) return e;
   return kv4::pick(a.c.d, a.c.groups, a.c.block_size, [&](auto d, auto ng, auto bs) {
     return kv4::launch_prefill<d, ng, bs>(p, grid, stream);
   });

@@ -862,7 +862,9 @@ torch::Tensor paged_prefill_kv4(torch::Tensor q, torch::Tensor cache, torch::Ten
   a.scale = (float)scale;
   const c10::cuda::CUDAGuard g(q.device());
   torch::Tensor out = torch::empty({T, hq, d}, q.options()), part;
+  torch::Tensor next = torch::empty({1}, q.options().dtype(at::kInt));
   a.out = out.data_ptr();
+  a.next = reinterpret_cast<unsigned*>(next.data_ptr<int>());
   const int64_t splits =
       es::kv4_prefill_splits(T, S, hq, a.c.hkv, std::min<int64_t>(max_context, block_tables.size(1) * block_size));
   a.max_splits = (int)splits;

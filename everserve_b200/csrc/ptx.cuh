@@ -77,6 +77,13 @@ ES_DEVICE void bulk_g2s(void* dst, const void* src, uint32_t bytes, uint64_t* ba
       : "memory");
 }
 
+// 16-byte asynchronous copy global -> shared of this thread (zeros where !valid), and the wait for all of them.
+ES_DEVICE void cp_async16(void* dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid ? 16 : 0)
+               : "memory");
+}
+ES_DEVICE void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 // An L2 policy for data read once per step (weights, the K/V history): its lines are the first
 // candidates for eviction, so streaming them does not push out lines fetched ahead for later use.
 ES_DEVICE uint64_t policy_evict_first() {
