@@ -579,20 +579,25 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
           vrun = ve;
         }
         // P times 2^(kPreBits + ve - vrun), back over the columns of S; the row's sum and the tile's maximum
-        float sum[4], mx[4];
+        float mx[4];
+        uint64_t sum[2];
+        const uint64_t cc = ptx::pair_f32(c, c);
         auto soft = [&](float add) {
           const float mc = (m == -INFINITY ? 0.f : -m) + add;
+          const uint64_t mm = ptx::pair_f32(mc, mc);
+          sum[0] = sum[1] = ptx::pair_f32(0.f, 0.f);
 #pragma unroll
-          for (int q = 0; q < 4; q++) sum[q] = 0.f, mx[q] = -INFINITY;
+          for (int q = 0; q < 4; q++) mx[q] = -INFINITY;
 #pragma unroll
           for (int q = 0; q < 4; q++) {
             uint32_t pk[16];
 #pragma unroll
             for (int i = 0; i < 16; i++) {
               const float x = __uint_as_float(v[q * 32 + 2 * i]), y = __uint_as_float(v[q * 32 + 2 * i + 1]);
-              const float a = ex2(fmaf(x, c, mc)), b = ex2(fmaf(y, c, mc));
+              const float2 e = ptx::unpair_f32(ptx::fma_f32x2(ptx::pair_f32(x, y), cc, mm));
+              const float a = ex2(e.x), b = ex2(e.y);
               mx[i & 3] = fmaxf(fmaxf(mx[i & 3], x), y);
-              sum[i & 3] += a + b;
+              sum[i & 1] = ptx::add_f32x2(sum[i & 1], ptx::pair_f32(a, b));
               const __half2 h = __floats2half2_rn(a, b);
               pk[i] = *reinterpret_cast<const uint32_t*>(&h);
             }
@@ -627,7 +632,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
         ptx::tmem_wait_st();
         ptx::tc_fence_before();
         ptx::mbar_arrive(&p_full[t]);
-        l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), ex2(-add), l);
+        const float2 both = ptx::unpair_f32(ptx::add_f32x2(sum[0], sum[1]));
+        l = fmaf(both.x + both.y, ex2(-add), l);
       }
       if (ok) ok = __all_sync(0xffffffffu, ptx::mbar_wait(&o_full[t], items & 1));
       if (!ok) break;

@@ -84,6 +84,28 @@ ES_DEVICE void cp_async16(void* dst, const void* src, bool valid) {
 }
 ES_DEVICE void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
+// Two fp32 operations in one instruction, on a pair of registers.
+ES_DEVICE uint64_t pair_f32(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+ES_DEVICE float2 unpair_f32(uint64_t d) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(d));
+  return f;
+}
+ES_DEVICE uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+ES_DEVICE uint64_t add_f32x2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
 // An L2 policy for data read once per step (weights, the K/V history): its lines are the first
 // candidates for eviction, so streaming them does not push out lines fetched ahead for later use.
 ES_DEVICE uint64_t policy_evict_first() {
