@@ -278,7 +278,7 @@ struct Kv4DecodeArgs {
   int64_t bt_stride, bt_cols;
   const int* ctx_lens;
   void* out;      // [B, hq, d]
-  float* part_o;  // [B, hq, max_splits, d] (unused with one split)
+  float* part_o;  // [B, hq, max_splits, d] (unused where kv4_decode_joins)
   float* part_ml; // [B, hq, max_splits, 2]
   int* status;
   int B, hq, max_splits;
@@ -286,6 +286,7 @@ struct Kv4DecodeArgs {
 };
 // splits a history of at most max_len positions is cut into (what part_o and part_ml are sized by)
 int64_t kv4_max_splits(int64_t max_len);
+bool kv4_decode_joins(int64_t max_splits);  // the kernel joins that many itself: no scratch
 cudaError_t launch_kv4_decode(const Kv4DecodeArgs& a, cudaStream_t s);
 // prefill: causal attention of T new rows of S sequences; sequence s owns the rows up to last_rows[s], the
 // last of them at position ctx_lens[s] - 1

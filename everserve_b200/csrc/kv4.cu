@@ -21,20 +21,37 @@ struct WriteParams {
   uint8_t* cache;
   int64_t s_block;  // bytes between blocks
   int64_t num_slots;
-  int64_t items;  // T * (hq + 2 hkv)
-  int hq, hkv;
+  int T, hq, hkv;
+  int share;  // log2 of the warps that share a token
   int* status;
 };
 
-// A quantised run of 8 channels as its word.
-ES_DEVICE uint32_t pack_word(const float* x, float scale, float zero) {
+// A quantised run of 8 channels as its word. A code is rint((x - zero) / scale) of the correctly rounded
+// quotient; the product with `inv`, the scale's rounded reciprocal, is within 15 * 2^-22 of it, so it gives the
+// same code unless it falls next to a half: then (1 word in 3000) the quotients are taken. The rounding is an
+// addition of 1.5 * 2^23, whose low bits are the code.
+ES_DEVICE uint32_t pack_word(const float* x, float scale, float zero, float inv) {
+  constexpr float kMagic = 12582912.f;
   uint32_t w = 0;
+  bool near = scale > 0.f && scale < 1e-30f;  // (a reciprocal that overflows)
+  const uint64_t z2 = ptx::pair_f32(-zero, -zero), m2 = ptx::pair_f32(kMagic, kMagic), n2 = ptx::pair_f32(-kMagic, -kMagic);
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    // the plain quotient, not a product with a reciprocal: a code is then what the formula says
-    const float c = scale > 0.f ? rintf(__fdiv_rn(x[i] - zero, scale)) : 0.f;
-    const uint32_t code = (uint32_t)fminf(fmaxf(c, 0.f), 15.f);
-    w |= code << (4 * (i / 2) + 16 * (i % 2));
+  for (int i = 0; i < 8; i += 2) {
+    const float2 d = ptx::unpair_f32(ptx::add_f32x2(ptx::pair_f32(x[i], x[i + 1]), z2));
+    const float q0 = fminf(fmaxf(d.x * inv, 0.f), 15.f), q1 = fminf(fmaxf(d.y * inv, 0.f), 15.f);
+    const uint64_t r2 = ptx::add_f32x2(ptx::pair_f32(q0, q1), m2);
+    const float2 r = ptx::unpair_f32(r2), c = ptx::unpair_f32(ptx::add_f32x2(r2, n2));
+    near |= fabsf(q0 - c.x) > 0.49998f || fabsf(q1 - c.y) > 0.49998f;
+    w += (__float_as_uint(r.x) - __float_as_uint(kMagic)) << (2 * i);
+    w += (__float_as_uint(r.y) - __float_as_uint(kMagic)) << (2 * i + 16);
+  }
+  if (near) {
+    w = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const float c = rintf(__fdiv_rn(x[i] - zero, scale));
+      w |= (uint32_t)fminf(fmaxf(c, 0.f), 15.f) << (4 * (i / 2) + 16 * (i % 2));
+    }
   }
   return w;
 }
@@ -45,115 +62,125 @@ ES_DEVICE uint32_t pack_word(const float* x, float scale, float zero) {
 // which are the two halves RoPE pairs, the two groups of a head in two groups, and (at D = 128) the two
 // words of one 8-byte piece of the row. A group's minimum and maximum are shuffles among these lanes.
 // The rotation rounds each product (no fused multiply-add), so a code does not depend on contraction.
+//
+// Bound by memory on paper (177 MB for 8190 rows of 48 heads: 27 us at the copy's rate), by instructions and
+// latency in fact: 43 us. A warp takes a token's heads, 32 / (D / 16) at a time, so the angles are read once;
+// 32 warps a SM (with four heads' loads at once and half the warps: 49 us; with IEEE quotients for every code: 60).
+// With few tokens several warps share one.
 template <int D, int NG, int BS>
-__global__ void __launch_bounds__(kThreads) write_kernel(WriteParams p) {
+__global__ void __launch_bounds__(kThreads, 4) write_kernel(WriteParams p) {
   using R = Rec<D, NG, BS>;
-  constexpr int L = D / 16;
+  constexpr int L = D / 16, H4 = 32 / L;  // lanes of a head, heads of a warp at a time
+  const int warp = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int t = warp >> p.share, part = warp & ((1 << p.share) - 1);
+  if (t >= p.T) return;
+  const int l = lane % L, H = p.hq + 2 * p.hkv, step = H4 << p.share;
   pdl_wait();
   pdl_launch();
-  const int64_t item0 = (int64_t)blockIdx.x * (kThreads / L) + threadIdx.x / L;
-  const bool live = item0 < p.items;
-  const int64_t item = live ? item0 : p.items - 1;
-  const int l = threadIdx.x % L;
-  const int H = p.hq + 2 * p.hkv;
-  const int64_t t = item / H;
-  const int h = (int)(item % H);
-  const __nv_bfloat16* src = p.qkv + t * p.qkv_stride + (int64_t)h * D;
-  float a[8], b[8];
-  unpack8(*reinterpret_cast<const uint4*>(src + 8 * l), a);
-  unpack8(*reinterpret_cast<const uint4*>(src + D / 2 + 8 * l), b);
-  if (p.bias != nullptr) {
-    float c[8];
-    unpack8(*reinterpret_cast<const uint4*>(p.bias + (int64_t)h * D + 8 * l), c);
-#pragma unroll
-    for (int i = 0; i < 8; i++) a[i] += c[i];
-    unpack8(*reinterpret_cast<const uint4*>(p.bias + (int64_t)h * D + D / 2 + 8 * l), c);
-#pragma unroll
-    for (int i = 0; i < 8; i++) b[i] += c[i];
-  }
-  if (h < p.hq + p.hkv) {
-    int64_t pos = p.positions[t];
-    if (pos < 0 || pos >= p.max_pos) {  // no table row: reported, and rotated as position 0
-      if (live && l == 0 && p.status) atomicExch(p.status, (int)kBadShape);
-      pos = 0;
-    }
+  int64_t pos = p.positions[t];
+  const int64_t slot = p.slots[t];
+  bool bad = slot >= p.num_slots;
+  if (pos < 0 || pos >= p.max_pos) bad = true, pos = 0;  // no table row: reported, and rotated as position 0
+  if (bad && lane == 0 && p.status) atomicExch(p.status, (int)kBadShape);
+  const bool kept = slot >= 0 && slot < p.num_slots;
+  float c[8], s[8];
+  {
     const float4* cs = reinterpret_cast<const float4*>(p.cos_sin + pos * D + 8 * l);
     const float4* sn = reinterpret_cast<const float4*>(p.cos_sin + pos * D + D / 2 + 8 * l);
     const float4 c0 = cs[0], c1 = cs[1], s0 = sn[0], s1 = sn[1];
-    const float c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-    const float s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+    c[0] = c0.x, c[1] = c0.y, c[2] = c0.z, c[3] = c0.w, c[4] = c1.x, c[5] = c1.y, c[6] = c1.z, c[7] = c1.w;
+    s[0] = s0.x, s[1] = s0.y, s[2] = s0.z, s[3] = s0.w, s[4] = s1.x, s[5] = s1.y, s[6] = s1.z, s[7] = s1.w;
+  }
+  const __nv_bfloat16* src = p.qkv + t * p.qkv_stride + 8 * l;
+  uint8_t* block = p.cache + (kept ? slot / BS : 0) * p.s_block;
+  const int off = (int)((kept ? slot : 0) % BS);
+  for (int base = part * H4; base < H; base += step) {
+    const int h = min(base + lane / L, H - 1);
+    const bool live = base + lane / L < H;
+    float a[8], b[8];
+    unpack8(__ldcs(reinterpret_cast<const uint4*>(src + h * D)), a);
+    unpack8(__ldcs(reinterpret_cast<const uint4*>(src + h * D + D / 2)), b);
+    if (p.bias != nullptr) {
+      float x[8];
+      unpack8(*reinterpret_cast<const uint4*>(p.bias + h * D + 8 * l), x);
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const float x = a[i], y = b[i];
-      a[i] = __fsub_rn(__fmul_rn(x, c[i]), __fmul_rn(y, s[i]));
-      b[i] = __fadd_rn(__fmul_rn(y, c[i]), __fmul_rn(x, s[i]));
+      for (int i = 0; i < 8; i++) a[i] += x[i];
+      unpack8(*reinterpret_cast<const uint4*>(p.bias + h * D + D / 2 + 8 * l), x);
+#pragma unroll
+      for (int i = 0; i < 8; i++) b[i] += x[i];
     }
-  }
-  // the groups' ranges (every lane shuffles; a query head's are not used)
-  float mn[2], mx[2], bad[2];  // bad: 0, or NaN where the group holds a value that is not finite
+    if (h < p.hq + p.hkv) {
 #pragma unroll
-  for (int g = 0; g < 2; g++) {
-    const float* x = g ? b : a;
-    mn[g] = mx[g] = x[0];
-    bad[g] = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      mn[g] = fminf(mn[g], x[i]);
-      mx[g] = fmaxf(mx[g], x[i]);
-      bad[g] += x[i] - x[i];
+      for (int i = 0; i < 8; i++) {
+        const float x = a[i], y = b[i];
+        a[i] = __fsub_rn(__fmul_rn(x, c[i]), __fmul_rn(y, s[i]));
+        b[i] = __fadd_rn(__fmul_rn(y, c[i]), __fmul_rn(x, s[i]));
+      }
     }
-  }
-  if (NG == 1) {
-    mn[0] = fminf(mn[0], mn[1]);
-    mx[0] = fmaxf(mx[0], mx[1]);
-    bad[0] += bad[1];
-  }
-#pragma unroll
-  for (int g = 0; g < NG; g++) {
-#pragma unroll
-    for (int o = 1; o < L; o <<= 1) {
-      mn[g] = fminf(mn[g], __shfl_xor_sync(0xffffffffu, mn[g], o));
-      mx[g] = fmaxf(mx[g], __shfl_xor_sync(0xffffffffu, mx[g], o));
-      bad[g] += __shfl_xor_sync(0xffffffffu, bad[g], o);
+    if (h < p.hq && live) {
+      uint4* q = reinterpret_cast<uint4*>(p.q_out + ((int64_t)t * p.hq + h) * D);
+      q[l] = pack8(a);
+      q[L + l] = pack8(b);
     }
-  }
-  if (!live) return;
-  if (h < p.hq) {
-    uint4* q = reinterpret_cast<uint4*>(p.q_out + (t * p.hq + h) * D);
-    q[l] = pack8(a);
-    q[L + l] = pack8(b);
-    return;
-  }
-  const int64_t slot = p.slots[t];
-  if (slot < 0) return;  // a padding row
-  if (slot >= p.num_slots) {
-    if (l == 0 && p.status) atomicExch(p.status, (int)kBadShape);
-    return;
-  }
-  const int side = h >= p.hq + p.hkv;  // 0: K, 1: V
-  const int kvh = h - p.hq - side * p.hkv;
-  uint8_t* rec = p.cache + (slot / BS) * p.s_block + (int64_t)kvh * R::kBytes;
-  const int off = (int)(slot % BS);
-  uint32_t pair = 0;  // lane l < NG stores the l-th group's
-  float s[NG], z[NG];
+    if (base + H4 <= p.hq || !kept) continue;  // query heads alone, or a padding row (the whole warp)
+    // the groups' ranges (every lane shuffles; a query head's are not used)
+    float mn[2], mx[2], bad[2];  // bad: 0, or NaN where the group holds a value that is not finite
 #pragma unroll
-  for (int g = 0; g < NG; g++) {
-    // a group holding a value that is not finite gets a NaN scale: all of it reads as NaN
-    const __nv_bfloat16 sb = f2bf(__fadd_rn(__fmul_rn(mx[g] - mn[g], 1.0f / 15.0f), bad[g]));
-    const __nv_bfloat16 zb = f2bf(mn[g]);
-    s[g] = bf2f(sb);
-    z[g] = bf2f(zb);
-    if (g == l) pair = (uint32_t)__bfloat16_as_ushort(sb) | ((uint32_t)__bfloat16_as_ushort(zb) << 16);
+    for (int g = 0; g < 2; g++) {
+      const float* x = g ? b : a;
+      mn[g] = mx[g] = x[0];
+#pragma unroll
+      for (int i = 1; i < 8; i++) {
+        mn[g] = fminf(mn[g], x[i]);
+        mx[g] = fmaxf(mx[g], x[i]);
+      }
+      uint64_t sum = ptx::pair_f32(0.f, 0.f);  // (scaled: it cannot overflow)
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        sum = ptx::fma_f32x2(ptx::pair_f32(x[2 * i], x[2 * i + 1]), ptx::pair_f32(0x1p-20f, 0x1p-20f), sum);
+      const float2 both = ptx::unpair_f32(sum);
+      bad[g] = (both.x + both.y) - (both.x + both.y);
+    }
+    if (NG == 1) {
+      mn[0] = fminf(mn[0], mn[1]);
+      mx[0] = fmaxf(mx[0], mx[1]);
+      bad[0] += bad[1];
+    }
+#pragma unroll
+    for (int g = 0; g < NG; g++) {
+#pragma unroll
+      for (int o = 1; o < L; o <<= 1) {
+        mn[g] = fminf(mn[g], __shfl_xor_sync(0xffffffffu, mn[g], o));
+        mx[g] = fmaxf(mx[g], __shfl_xor_sync(0xffffffffu, mx[g], o));
+        bad[g] += __shfl_xor_sync(0xffffffffu, bad[g], o);
+      }
+    }
+    if (!live || h < p.hq) continue;
+    const int side = h >= p.hq + p.hkv;  // 0: K, 1: V
+    uint8_t* rec = block + (h - p.hq - side * p.hkv) * R::kBytes;
+    uint32_t pair = 0;  // lane l < NG stores the l-th group's
+    float sc[NG], z[NG], inv[NG];
+#pragma unroll
+    for (int g = 0; g < NG; g++) {
+      // a group holding a value that is not finite gets a NaN scale: all of it reads as NaN
+      const __nv_bfloat16 sb = f2bf(__fadd_rn(__fmul_rn(mx[g] - mn[g], 1.0f / 15.0f), bad[g]));
+      const __nv_bfloat16 zb = f2bf(mn[g]);
+      sc[g] = bf2f(sb);
+      z[g] = bf2f(zb);
+      inv[g] = sc[g] > 0.f ? __frcp_rn(sc[g]) : 0.f;
+      if (g == l) pair = (uint32_t)__bfloat16_as_ushort(sb) | ((uint32_t)__bfloat16_as_ushort(zb) << 16);
+    }
+    const uint32_t wa = pack_word(a, sc[0], z[0], inv[0]);
+    const uint32_t wb = pack_word(b, sc[NG - 1], z[NG - 1], inv[NG - 1]);
+    uint8_t* row = rec + side * R::kV + off * R::kRow;
+    if (D == 128) {
+      *reinterpret_cast<uint2*>(row + 8 * l) = make_uint2(wa, wb);
+    } else {
+      *reinterpret_cast<uint32_t*>(row + 4 * l) = wa;
+      *reinterpret_cast<uint32_t*>(row + R::kRow / 2 + 4 * l) = wb;
+    }
+    if (l < NG) *reinterpret_cast<uint32_t*>(rec + R::kKMeta + side * BS * R::kMeta + off * R::kMeta + 4 * l) = pair;
   }
-  const uint32_t wa = pack_word(a, s[0], z[0]), wb = pack_word(b, s[NG - 1], z[NG - 1]);
-  uint8_t* row = rec + side * R::kV + off * R::kRow;
-  if (D == 128) {
-    *reinterpret_cast<uint2*>(row + 8 * l) = make_uint2(wa, wb);
-  } else {
-    *reinterpret_cast<uint32_t*>(row + 4 * l) = wa;
-    *reinterpret_cast<uint32_t*>(row + R::kRow / 2 + 4 * l) = wb;
-  }
-  if (l < NG) *reinterpret_cast<uint32_t*>(rec + R::kKMeta + side * BS * R::kMeta + off * R::kMeta + 4 * l) = pair;
 }
 
 struct ReadParams {
@@ -161,8 +188,7 @@ struct ReadParams {
   int64_t s_block, num_slots;
   const int64_t* slots;
   __nv_bfloat16 *k, *v;  // [n, hkv, D]
-  int64_t items;         // n * hkv * 2
-  int hkv;
+  uint32_t items, hkv;   // n * hkv
   int* status;
 };
 
@@ -174,40 +200,44 @@ __global__ void __launch_bounds__(kThreads) read_kernel(ReadParams p) {
   constexpr int L = D / 16;
   pdl_wait();
   pdl_launch();
-  const int64_t item = (int64_t)blockIdx.x * (kThreads / L) + threadIdx.x / L;
+  const uint32_t item = blockIdx.x * (kThreads / L) + threadIdx.x / L;  // (token, kv head)
   if (item >= p.items) return;
   const int l = threadIdx.x % L;
-  const int side = (int)(item & 1);
-  const int64_t row = item >> 1;  // token * hkv + kv head
-  const int64_t slot = p.slots[row / p.hkv];
-  float a[8], b[8];
-#pragma unroll
-  for (int i = 0; i < 8; i++) a[i] = b[i] = 0.f;  // a negative slot reads as zeros
-  if (slot >= p.num_slots) {
-    if (l == 0 && p.status) atomicExch(p.status, (int)kBadShape);
-  } else if (slot >= 0) {
-    const uint8_t* rec = p.cache + (slot / BS) * p.s_block + (row % p.hkv) * R::kBytes;
+  const uint32_t t = item / p.hkv;
+  const int64_t slot = p.slots[t];
+  const bool in = slot >= 0 && slot < p.num_slots;  // a negative slot reads as zeros
+  if (slot >= p.num_slots && l == 0 && p.status) atomicExch(p.status, (int)kBadShape);
+  uint2 w[2];
+  uint32_t pa[2], pb[2];
+  if (in) {
+    const uint8_t* rec = p.cache + slot / BS * p.s_block + (item - t * p.hkv) * R::kBytes;
     const int off = (int)(slot % BS);
-    const uint8_t* codes = rec + side * R::kV + off * R::kRow;
-    const uint32_t* pair = reinterpret_cast<const uint32_t*>(rec + R::kKMeta + side * BS * R::kMeta + off * R::kMeta);
-    uint2 w;
-    if (D == 128) {
-      w = *reinterpret_cast<const uint2*>(codes + 8 * l);
-    } else {
-      w.x = *reinterpret_cast<const uint32_t*>(codes + 4 * l);
-      w.y = *reinterpret_cast<const uint32_t*>(codes + R::kRow / 2 + 4 * l);
+#pragma unroll
+    for (int side = 0; side < 2; side++) {
+      const uint8_t* codes = rec + side * R::kV + off * R::kRow;
+      const uint32_t* pair = reinterpret_cast<const uint32_t*>(rec + R::kKMeta + side * BS * R::kMeta + off * R::kMeta);
+      if (D == 128) {
+        w[side] = *reinterpret_cast<const uint2*>(codes + 8 * l);
+      } else {
+        w[side].x = *reinterpret_cast<const uint32_t*>(codes + 4 * l);
+        w[side].y = *reinterpret_cast<const uint32_t*>(codes + R::kRow / 2 + 4 * l);
+      }
+      pa[side] = pair[0], pb[side] = pair[NG - 1];
     }
-    const uint32_t pa = pair[0], pb = pair[NG - 1];
+  }
+#pragma unroll
+  for (int side = 0; side < 2; side++) {
+    float a[8], b[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) {
       const int bit = 4 * (i / 2) + 16 * (i % 2);
-      a[i] = fmaf((float)((w.x >> bit) & 15u), pair_scale(pa), pair_zero(pa));
-      b[i] = fmaf((float)((w.y >> bit) & 15u), pair_scale(pb), pair_zero(pb));
+      a[i] = in ? fmaf((float)((w[side].x >> bit) & 15u), pair_scale(pa[side]), pair_zero(pa[side])) : 0.f;
+      b[i] = in ? fmaf((float)((w[side].y >> bit) & 15u), pair_scale(pb[side]), pair_zero(pb[side])) : 0.f;
     }
+    uint4* dst = reinterpret_cast<uint4*>((side ? p.v : p.k) + (int64_t)item * D);
+    dst[l] = pack8(a);
+    dst[L + l] = pack8(b);
   }
-  uint4* dst = reinterpret_cast<uint4*>((side ? p.v : p.k) + row * D);
-  dst[l] = pack8(a);
-  dst[L + l] = pack8(b);
 }
 
 // ---- pages ---------------------------------------------------------------------------------------
@@ -272,12 +302,15 @@ cudaError_t launch_rope_kv4(const Kv4WriteArgs& a, cudaStream_t stream) {
   p.num_slots = a.c.num_blocks * a.c.block_size;
   p.hq = a.hq;
   p.hkv = a.c.hkv;
-  p.items = a.T * (a.hq + 2 * a.c.hkv);
+  p.T = (int)a.T;
   p.status = a.status;
-  if (p.items == 0) return cudaSuccess;
+  if (a.T == 0) return cudaSuccess;
+  if (a.T > INT32_MAX / 64 || (int64_t)(a.hq + 2 * a.c.hkv) * a.c.d > INT32_MAX) return cudaErrorInvalidValue;
   return kv4::pick(a.c.d, a.c.groups, a.c.block_size, [&](auto d, auto ng, auto bs) {
-    const int64_t grid = (p.items + kv4::kThreads / (d / 16) - 1) / (kv4::kThreads / (d / 16));
-    if (grid > INT32_MAX) return cudaErrorInvalidValue;
+    // as many warps to a token (a power of two) as its heads fill, while the tokens alone do not fill the SMs
+    const int fill = (a.hq + 2 * a.c.hkv + 32 / (d / 16) - 1) / (32 / (d / 16));
+    while (p.share < 5 && (1 << p.share) < fill && (a.T << p.share) < 2048) p.share++;
+    const int64_t grid = ((a.T << p.share) + kv4::kThreads / 32 - 1) / (kv4::kThreads / 32);
     return launch_ex(kv4::write_kernel<d, ng, bs>, dim3((unsigned)grid), dim3(kv4::kThreads), 0, stream, 0, p);
   });
 }
@@ -291,12 +324,12 @@ cudaError_t launch_kv4_read(const Kv4ReadArgs& a, cudaStream_t stream) {
   p.k = static_cast<__nv_bfloat16*>(a.k);
   p.v = static_cast<__nv_bfloat16*>(a.v);
   p.hkv = a.c.hkv;
-  p.items = a.n * a.c.hkv * 2;
   p.status = a.status;
-  if (p.items == 0) return cudaSuccess;
+  if (a.n == 0) return cudaSuccess;
+  if (a.n * a.c.hkv > INT32_MAX) return cudaErrorInvalidValue;
+  p.items = (uint32_t)(a.n * a.c.hkv);
   return kv4::pick(a.c.d, a.c.groups, a.c.block_size, [&](auto d, auto ng, auto bs) {
-    const int64_t grid = (p.items + kv4::kThreads / (d / 16) - 1) / (kv4::kThreads / (d / 16));
-    if (grid > INT32_MAX) return cudaErrorInvalidValue;
+    const int64_t grid = ((int64_t)p.items + kv4::kThreads / (d / 16) - 1) / (kv4::kThreads / (d / 16));
     return launch_ex(kv4::read_kernel<d, ng, bs>, dim3((unsigned)grid), dim3(kv4::kThreads), 0, stream, 0, p);
   });
 }

@@ -19,8 +19,9 @@
 // A warp takes one (sequence, kv head, split of the history) by itself: the records of its blocks stream
 // through a ring of its own in shared memory, one bulk copy a block, and nothing but that ring's barriers
 // is waited for. The running maximum moves only when a score passes it by 2^6 (a vote per 16 keys; the
-// first ones set it), so most runs shuffle nothing. A second kernel joins the splits. How a history is
-// cut depends on its length alone: a sequence's result does not depend on the batch.
+// first ones set it), so most runs shuffle nothing. The splits of a pair are neighbouring warps: where a CTA
+// holds all of them (histories up to 2048 keys) it joins them itself, else a second kernel does, in the same
+// order. How a history is cut depends on its length alone: a sequence's result does not depend on the batch.
 #include <algorithm>
 #include <atomic>
 
@@ -34,7 +35,7 @@ namespace kv4 {
 
 constexpr int kDecWarps = 4;
 constexpr int kDecThreads = kDecWarps * 32;
-constexpr int kDecCtas = 4;  // a SM
+constexpr int kDecCtas = 4;  // a SM (8 warps and 2 CTAs: 62 us against 56 for 48 ragged sequences)
 constexpr float kLog2eF = 1.4426950408889634f;
 constexpr float kSlack = 6.f;       // log2 of how far a score may pass the running maximum
 constexpr int kPBits = 7;           // P * scale enters f16 as at most 2^(6 + 2 + 7) = 2^15
@@ -71,6 +72,7 @@ struct DecodeParams {
   float* part_ml;
   int* status;
   int hq, hkv, head_tiles, max_splits;
+  int join;  // a pair's splits are one CTA's, which joins them
   float scale_log2;
 };
 
@@ -299,6 +301,47 @@ ES_DEVICE void attend(Acc<D, NG>& A, const Query<D, NG>& Q, bool first, const ui
   }
 }
 
+// out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i over a row's splits. A row of at most kFew splits is one
+// warp's, in order; a longer one is a CTA's: warp w takes splits w, w + 8, ..., then the warps add in order.
+// (The rule is the row's own count, so its bits do not depend on the launch.) Four splits' loads are on the
+// way at a time.
+constexpr int kMergeWarps = 8;
+constexpr int kFew = 16;
+
+template <int D>
+struct Part {
+  static constexpr int E = D / 32;  // neighbouring channels of a lane
+  float acc[E], l;
+  // splits first, first + step, ... of a row whose maximum is mx; po(i), ml(i): split i's output and (m, l)
+  template <typename O, typename M>
+  ES_DEVICE void sum(O&& po, M&& ml, int ns, int first, int step, float mx, int lane) {
+    l = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; e++) acc[e] = 0.f;
+#pragma unroll 4
+    for (int i = first; i < ns; i += step) {
+      const float2 t = ml(i);
+      const float f = t.x == mx ? 1.f : ex2(t.x - mx);
+      l = fmaf(t.y, f, l);
+      float v[E];
+      if (E == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(po(i) + E * lane);
+        v[0] = x.x, v[1] = x.y, v[E - 2] = x.z, v[E - 1] = x.w;
+      } else {
+        const float2 x = *reinterpret_cast<const float2*>(po(i) + E * lane);
+        v[0] = x.x, v[1] = x.y;
+      }
+#pragma unroll
+      for (int e = 0; e < E; e++) acc[e] = fmaf(v[e], f, acc[e]);
+    }
+  }
+  ES_DEVICE void write(__nv_bfloat16* out, int lane) const {
+#pragma unroll
+    for (int e = 0; e < E; e += 2)
+      *reinterpret_cast<__nv_bfloat162*>(out + E * lane + e) = __floats2bfloat162_rn(acc[e] / l, acc[e + 1] / l);
+  }
+};
+
 template <int D, int NG, int BS>
 __global__ void __launch_bounds__(kDecThreads, kDecCtas) decode_kernel(DecodeParams p) {
   using R = Rec<D, NG, BS>;
@@ -317,6 +360,7 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas) decode_kernel(DecodePar
   const int gid = lane >> 2, tig = lane & 3;
   uint8_t* ring = smem + warp * C::kBytes;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + kDecWarps * C::kBytes) + warp * ST;
+  float* own_o = reinterpret_cast<float*>(ring);  // [8][D] and (m, l) [8], once the ring is done with
   if (lane == 0) {
     for (int i = 0; i < ST; i++) ptx::mbar_init(&full[i], 1);
     ptx::fence_mbar_init();
@@ -326,200 +370,179 @@ __global__ void __launch_bounds__(kDecThreads, kDecCtas) decode_kernel(DecodePar
   pdl_wait();
   pdl_launch();
   const int ctx = min(p.ctx_lens[b], p.bt_cols * BS);
-  if (ctx <= 0) {
-    if (split == 0)  // an empty history: the output is zero
-      for (int i = lane; i < heads * D; i += 32) p.out[((int64_t)b * p.hq + head0) * D + i] = f2bf(0.f);
-    return;
-  }
   const int ns = min(p.max_splits, splits_of(ctx));
-  const int plen = ((ctx + ns - 1) / ns + BS - 1) / BS * BS;  // equal splits, to a block
-  const int s0 = split * plen, s1 = min(ctx, s0 + plen);
-  if (split >= ns) return;
   const int64_t row0 = (int64_t)b * p.hq + head0;
-  const int blocks = (s1 - s0 + BS - 1) / BS;
-
-  // the block table's entries, 32 at a time, one a lane
-  const int* bt = p.block_tables + (int64_t)b * p.bt_stride + s0 / BS;
-  auto entries = [&](int first) {
-    int64_t blk = first + lane < blocks ? bt[first + lane] : 0;
-    if (blk < 0 || blk >= p.num_blocks) {  // not a block of this cache: reported, block 0 read instead
-      if (p.status) atomicExch(p.status, (int)kBadShape);
-      blk = 0;
-    }
-    return (int)blk;
-  };
-  int ids = entries(0);
-  const uint8_t* head_base = p.cache + (int64_t)kvh * R::kBytes;
-  const uint64_t pol = ptx::policy_evict_first();
-  int issued = 0;  // blocks whose copies are on the way or done
-  auto issue = [&](int stage) {  // the next step's
-    if (issued != 0 && (issued & 31) == 0) ids = entries(issued);
-    const int n = min(PB, blocks - issued);
-    const int64_t b0 = __shfl_sync(0xffffffffu, ids, issued & 31), b1 = __shfl_sync(0xffffffffu, ids, (issued + PB - 1) & 31);
-    if (lane == 0) {
-      ptx::mbar_arrive_expect_tx(&full[stage], n * R::kBytes);
-      uint8_t* dst = ring + stage * PB * R::kBytes;
-      ptx::bulk_g2s_hint(dst, head_base + b0 * p.s_block, R::kBytes, &full[stage], pol);
-      if (n == 2) ptx::bulk_g2s_hint(dst + R::kBytes, head_base + b1 * p.s_block, R::kBytes, &full[stage], pol);
-    }
-    issued += n;
-  };
-  for (int i = 0; i < ST && issued < blocks; i++) issue(i);
-
-  // the query, scaled to <= 2^10
-  Query<D, NG> Q;
-  {
-    float qv[KW][8];
-    float qmax = 0.f, sum[2] = {0.f, 0.f};
-    const __nv_bfloat16* qr = p.q + (int64_t)b * p.q_stride + (int64_t)(head0 + min(gid, heads - 1)) * D;
-#pragma unroll
-    for (int w = 0; w < KW; w++) {
-      const int pos = tig * KW + w;  // stored word of the row, and the channels it holds
-      const int nat = D == 128 ? (pos >> 1) + 8 * (pos & 1) : pos;
-      unpack8(*reinterpret_cast<const uint4*>(qr + 8 * nat), qv[w]);
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        if (gid >= heads) qv[w][i] = 0.f;
-        qmax = fmaxf(qmax, fabsf(qv[w][i]));
-        sum[NG == 2 ? (w & 1) : 1] += qv[w][i];
-      }
-    }
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-      qmax = fmaxf(qmax, __shfl_xor_sync(0xffffffffu, qmax, o));
-#pragma unroll
-      for (int g = 0; g < 2; g++) sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], o);
-    }
-    const int e = exponent(qmax);
-    const float f = pow2i(9 - e), f16th = f * 0.0625f;
-#pragma unroll
-    for (int w = 0; w < KW; w++) {
-      Q.b[w][0] = pack_f16x2(qv[w][0] * f, qv[w][1] * f);
-      Q.b[w][1] = pack_f16x2(qv[w][2] * f16th, qv[w][3] * f16th);
-      Q.b[w][2] = pack_f16x2(qv[w][4] * f, qv[w][5] * f);
-      Q.b[w][3] = pack_f16x2(qv[w][6] * f16th, qv[w][7] * f16th);
-    }
-    const float x = p.scale_log2 * pow2i(24 - 9 + e);
-#pragma unroll
-    for (int i = 0; i < 2; i++) Q.xs[i] = __shfl_sync(0xffffffffu, x, (2 * tig + i) * 4);
-    // scale * sum q in three terms of 8 bits, lane tig the tig-th: (first group, second), or with one group
-    // (0, the sum), which meets (scale, zero) of a key as stored
-    float t[2] = {p.scale_log2 * sum[0], p.scale_log2 * sum[1]};
-#pragma unroll
-    for (int i = 0; i < 2; i++)
-      if (i < tig) t[0] -= bf2f(f2bf(t[0])), t[1] -= bf2f(f2bf(t[1]));
-    Q.zero = tig < 3 ? ptx::pack_bf16x2(t[0], t[1]) : 0u;
-  }
-
-  Acc<D, NG> A;
-#pragma unroll
-  for (int i = 0; i < D / 16; i++) A.o[i][0] = A.o[i][1] = A.o[i][2] = A.o[i][3] = 0.f;
-#pragma unroll
-  for (int j = 0; j < 2; j++) {
-    A.m[j] = 0.f, A.l[j] = 0.f;
-#pragma unroll
-    for (int g = 0; g < NG; g++) A.zs[j][g] = 0.f;
-  }
-  A.k = 0.f;
-  A.vlim = 0.f;
-
-  int stage = 0, phase = 0;
-  for (int i = 0; i < blocks; i += PB) {
-    if (!__all_sync(0xffffffffu, ptx::mbar_wait(&full[stage], phase))) {
-      // the copies on their way have to land before the warp leaves
-      for (int k = i / PB; k * PB < issued; k++) ptx::mbar_wait(&full[k % ST], (k / ST) & 1);
-      if (lane == 0 && p.status) atomicExch(p.status, (int)kTimeout);
+  auto attend_split = [&]() {
+    if (ctx <= 0) {
+      if (split == 0)  // an empty history: the output is zero
+        for (int i = lane; i < heads * D; i += 32) p.out[((int64_t)b * p.hq + head0) * D + i] = f2bf(0.f);
       return;
     }
-    const uint8_t* rec0 = ring + stage * PB * R::kBytes;
-    const uint8_t* rec1 = PB == 2 ? rec0 + R::kBytes : rec0;  // (of a block the split lacks: not counted)
-    const int valid = s1 - s0 - i * BS;
-    if (valid >= 32)
-      attend<D, NG, BS, false>(A, Q, i == 0, rec0, rec1, 2 - PB, gid, tig, 32);
-    else
-      attend<D, NG, BS, true>(A, Q, i == 0, rec0, rec1, 2 - PB, gid, tig, valid);
-    __syncwarp();  // every lane has read the step's stage
-    if (issued < blocks) issue(stage);
-    if (++stage == ST) stage = 0, phase ^= 1;
-  }
+    const int plen = ((ctx + ns - 1) / ns + BS - 1) / BS * BS;  // equal splits, to a block
+    const int s0 = split * plen, s1 = min(ctx, s0 + plen);
+    if (split >= ns) return;
+    const int blocks = (s1 - s0 + BS - 1) / BS;
 
-  // the lanes' sums; the output with the codes' factor and the zeros' part
+    // the block table's entries, 32 at a time, one a lane
+    const int* bt = p.block_tables + (int64_t)b * p.bt_stride + s0 / BS;
+    auto entries = [&](int first) {
+      int64_t blk = first + lane < blocks ? bt[first + lane] : 0;
+      if (blk < 0 || blk >= p.num_blocks) {  // not a block of this cache: reported, block 0 read instead
+        if (p.status) atomicExch(p.status, (int)kBadShape);
+        blk = 0;
+      }
+      return (int)blk;
+    };
+    int ids = entries(0);
+    const uint8_t* head_base = p.cache + (int64_t)kvh * R::kBytes;
+    const uint64_t pol = ptx::policy_evict_first();
+    int issued = 0;  // blocks whose copies are on the way or done
+    auto issue = [&](int stage) {  // the next step's
+      if (issued != 0 && (issued & 31) == 0) ids = entries(issued);
+      const int n = min(PB, blocks - issued);
+      const int64_t b0 = __shfl_sync(0xffffffffu, ids, issued & 31), b1 = __shfl_sync(0xffffffffu, ids, (issued + PB - 1) & 31);
+      if (lane == 0) {
+        ptx::mbar_arrive_expect_tx(&full[stage], n * R::kBytes);
+        uint8_t* dst = ring + stage * PB * R::kBytes;
+        ptx::bulk_g2s_hint(dst, head_base + b0 * p.s_block, R::kBytes, &full[stage], pol);
+        if (n == 2) ptx::bulk_g2s_hint(dst + R::kBytes, head_base + b1 * p.s_block, R::kBytes, &full[stage], pol);
+      }
+      issued += n;
+    };
+    for (int i = 0; i < ST && issued < blocks; i++) issue(i);
+
+    // the query, scaled to <= 2^10
+    Query<D, NG> Q;
+    {
+      float qv[KW][8];
+      float qmax = 0.f, sum[2] = {0.f, 0.f};
+      const __nv_bfloat16* qr = p.q + (int64_t)b * p.q_stride + (int64_t)(head0 + min(gid, heads - 1)) * D;
 #pragma unroll
-  for (int s = 4; s < 32; s <<= 1) {
+      for (int w = 0; w < KW; w++) {
+        const int pos = tig * KW + w;  // stored word of the row, and the channels it holds
+        const int nat = D == 128 ? (pos >> 1) + 8 * (pos & 1) : pos;
+        unpack8(*reinterpret_cast<const uint4*>(qr + 8 * nat), qv[w]);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          if (gid >= heads) qv[w][i] = 0.f;
+          qmax = fmaxf(qmax, fabsf(qv[w][i]));
+          sum[NG == 2 ? (w & 1) : 1] += qv[w][i];
+        }
+      }
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {
+        qmax = fmaxf(qmax, __shfl_xor_sync(0xffffffffu, qmax, o));
+#pragma unroll
+        for (int g = 0; g < 2; g++) sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], o);
+      }
+      const int e = exponent(qmax);
+      const float f = pow2i(9 - e), f16th = f * 0.0625f;
+#pragma unroll
+      for (int w = 0; w < KW; w++) {
+        Q.b[w][0] = pack_f16x2(qv[w][0] * f, qv[w][1] * f);
+        Q.b[w][1] = pack_f16x2(qv[w][2] * f16th, qv[w][3] * f16th);
+        Q.b[w][2] = pack_f16x2(qv[w][4] * f, qv[w][5] * f);
+        Q.b[w][3] = pack_f16x2(qv[w][6] * f16th, qv[w][7] * f16th);
+      }
+      const float x = p.scale_log2 * pow2i(24 - 9 + e);
+#pragma unroll
+      for (int i = 0; i < 2; i++) Q.xs[i] = __shfl_sync(0xffffffffu, x, (2 * tig + i) * 4);
+      // scale * sum q in three terms of 8 bits, lane tig the tig-th: (first group, second), or with one group
+      // (0, the sum), which meets (scale, zero) of a key as stored
+      float t[2] = {p.scale_log2 * sum[0], p.scale_log2 * sum[1]};
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+        if (i < tig) t[0] -= bf2f(f2bf(t[0])), t[1] -= bf2f(f2bf(t[1]));
+      Q.zero = tig < 3 ? ptx::pack_bf16x2(t[0], t[1]) : 0u;
+    }
+
+    Acc<D, NG> A;
+#pragma unroll
+    for (int i = 0; i < D / 16; i++) A.o[i][0] = A.o[i][1] = A.o[i][2] = A.o[i][3] = 0.f;
 #pragma unroll
     for (int j = 0; j < 2; j++) {
-      A.l[j] += __shfl_xor_sync(0xffffffffu, A.l[j], s);
+      A.m[j] = 0.f, A.l[j] = 0.f;
 #pragma unroll
-      for (int g = 0; g < NG; g++) A.zs[j][g] += __shfl_xor_sync(0xffffffffu, A.zs[j][g], s);
+      for (int g = 0; g < NG; g++) A.zs[j][g] = 0.f;
     }
-  }
+    A.k = 0.f;
+    A.vlim = 0.f;
+
+    int stage = 0, phase = 0;
+    for (int i = 0; i < blocks; i += PB) {
+      if (!__all_sync(0xffffffffu, ptx::mbar_wait(&full[stage], phase))) {
+        // the copies on their way have to land before the warp leaves
+        for (int k = i / PB; k * PB < issued; k++) ptx::mbar_wait(&full[k % ST], (k / ST) & 1);
+        if (lane == 0 && p.status) atomicExch(p.status, (int)kTimeout);
+        return;
+      }
+      const uint8_t* rec0 = ring + stage * PB * R::kBytes;
+      const uint8_t* rec1 = PB == 2 ? rec0 + R::kBytes : rec0;  // (of a block the split lacks: not counted)
+      const int valid = s1 - s0 - i * BS;
+      if (valid >= 32)
+        attend<D, NG, BS, false>(A, Q, i == 0, rec0, rec1, 2 - PB, gid, tig, 32);
+      else
+        attend<D, NG, BS, true>(A, Q, i == 0, rec0, rec1, 2 - PB, gid, tig, valid);
+      __syncwarp();  // every lane has read the step's stage
+      if (issued < blocks) issue(stage);
+      if (++stage == ST) stage = 0, phase ^= 1;
+    }
+
+    // the lanes' sums; the output with the codes' factor and the zeros' part
 #pragma unroll
-  for (int j = 0; j < 2; j++) {
-    const int h = 2 * tig + j;
-    if (h >= heads) continue;
-    const float inv = 1.f / A.l[j];
+    for (int s = 4; s < 32; s <<= 1) {
 #pragma unroll
-    for (int w = 0; w < VW; w++) {
-      float y[8];  // channels 8 (gid + 8 w) and up
-      const float z = A.zs[j][NG == 2 ? w : 0];
+      for (int j = 0; j < 2; j++) {
+        A.l[j] += __shfl_xor_sync(0xffffffffu, A.l[j], s);
 #pragma unroll
-      for (int i = 0; i < 4; i += 2)
-#pragma unroll
-        for (int c = 0; c < 2; c++) {
-          const float odd = A.o[w * 4 + i + 1][2 * c + j], even = A.o[w * 4 + i][2 * c + j] - odd;
-          y[2 * i + c] = fmaf(even, 16777216.f, z);         // 2^24: a code in bits 0..3
-          y[2 * i + 2 + c] = fmaf(odd, 1048576.f, z);       // 2^20: in bits 4..7
-        }
-      const int ch = 8 * (gid + 8 * w);
-      if (ns == 1) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) y[i] *= inv;
-        *reinterpret_cast<uint4*>(p.out + (row0 + h) * D + ch) = pack8(y);
-      } else {
-        float4* po = reinterpret_cast<float4*>(p.part_o + ((row0 + h) * p.max_splits + split) * D + ch);
-        po[0] = make_float4(y[0], y[1], y[2], y[3]);
-        po[1] = make_float4(y[4], y[5], y[6], y[7]);
+        for (int g = 0; g < NG; g++) A.zs[j][g] += __shfl_xor_sync(0xffffffffu, A.zs[j][g], s);
       }
     }
-    if (ns > 1 && gid == 0)
-      *reinterpret_cast<float2*>(p.part_ml + ((row0 + h) * p.max_splits + split) * 2) = make_float2(A.m[j] - A.k, A.l[j]);
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      const int h = 2 * tig + j;
+      if (h >= heads) continue;
+      const float inv = 1.f / A.l[j];
+#pragma unroll
+      for (int w = 0; w < VW; w++) {
+        float y[8];  // channels 8 (gid + 8 w) and up
+        const float z = A.zs[j][NG == 2 ? w : 0];
+#pragma unroll
+        for (int i = 0; i < 4; i += 2)
+#pragma unroll
+          for (int c = 0; c < 2; c++) {
+            const float odd = A.o[w * 4 + i + 1][2 * c + j], even = A.o[w * 4 + i][2 * c + j] - odd;
+            y[2 * i + c] = fmaf(even, 16777216.f, z);         // 2^24: a code in bits 0..3
+            y[2 * i + 2 + c] = fmaf(odd, 1048576.f, z);       // 2^20: in bits 4..7
+          }
+        const int ch = 8 * (gid + 8 * w);
+        if (ns == 1) {
+#pragma unroll
+          for (int i = 0; i < 8; i++) y[i] *= inv;
+          *reinterpret_cast<uint4*>(p.out + (row0 + h) * D + ch) = pack8(y);
+        } else {
+          float4* po = reinterpret_cast<float4*>(p.join ? own_o + h * D + ch : p.part_o + ((row0 + h) * p.max_splits + split) * D + ch);
+          po[0] = make_float4(y[0], y[1], y[2], y[3]);
+          po[1] = make_float4(y[4], y[5], y[6], y[7]);
+        }
+      }
+      if (ns > 1 && gid == 0)
+        *(p.join ? reinterpret_cast<float2*>(own_o + 8 * D) + h
+                 : reinterpret_cast<float2*>(p.part_ml) + (row0 + h) * p.max_splits + split) = make_float2(A.m[j] - A.k, A.l[j]);
+    }
+  };
+  attend_split();
+  if (!p.join || ctx <= 0 || ns == 1) return;
+  // the splits' results, in the warps' own rings, joined a warp a query head
+  __syncthreads();
+  for (int h = warp; h < heads; h += kDecWarps) {
+    Part<D> a;
+    auto ml = [&](int i) { return reinterpret_cast<const float2*>(smem + i * C::kBytes + 8 * D * 4)[h]; };
+    const float mx = warp_max(lane < ns ? ml(lane).x : -INFINITY);
+    a.sum([&](int i) { return reinterpret_cast<const float*>(smem + i * C::kBytes) + h * D; }, ml, ns, 0, 1, mx, lane);
+    a.write(p.out + (row0 + h) * D, lane);
   }
 }
-
-// out = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i over a row's splits. A row of at most kFew splits is one
-// warp's, in order; a longer one is a CTA's: warp w takes splits w, w + 8, ..., then the warps add in order.
-// (The rule is the row's own count, so its bits do not depend on the launch.) Four splits' loads are on the
-// way at a time.
-constexpr int kMergeWarps = 8;
-constexpr int kFew = 16;
-
-template <int D>
-struct Part {
-  static constexpr int E = D / 32;  // neighbouring channels of a lane
-  float acc[E], l;
-  // splits first, first + step, ... of a row whose maximum is mx
-  ES_DEVICE void sum(const float* po, const float2* ml, int ns, int first, int step, float mx, int lane) {
-    l = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; e++) acc[e] = 0.f;
-#pragma unroll 4
-    for (int i = first; i < ns; i += step) {
-      const float2 t = ml[i];
-      const float f = t.x == mx ? 1.f : ex2(t.x - mx);
-      l = fmaf(t.y, f, l);
-      float v[E];
-      if (E == 4) {
-        const float4 x = *reinterpret_cast<const float4*>(po + (int64_t)i * D + E * lane);
-        v[0] = x.x, v[1] = x.y, v[E - 2] = x.z, v[E - 1] = x.w;
-      } else {
-        const float2 x = *reinterpret_cast<const float2*>(po + (int64_t)i * D + E * lane);
-        v[0] = x.x, v[1] = x.y;
-      }
-#pragma unroll
-      for (int e = 0; e < E; e++) acc[e] = fmaf(v[e], f, acc[e]);
-    }
-  }
-};
 
 // kRows: a CTA takes kMergeWarps rows, a warp each (no row has more than kFew splits); else one row.
 template <int D, bool kRows>
@@ -535,20 +558,19 @@ __global__ void __launch_bounds__(kMergeWarps * 32)
   if (row >= rows) return;
   const int ns = min(max_splits, splits_of(min(ctx_lens[row / hq], max_keys)));
   if (ns <= 1) return;  // written by the split itself
-  const float2* ml = reinterpret_cast<const float2*>(part_ml) + row * max_splits;
-  const float* po = part_o + row * max_splits * D;
+  auto ml = [&](int i) { return reinterpret_cast<const float2*>(part_ml)[row * max_splits + i]; };
+  auto po = [&](int i) { return part_o + (row * max_splits + i) * D; };
   Part<D> a;
   if (ns <= kFew) {
     if (!kRows && warp > 0) return;
-    const float mx = warp_max(lane < ns ? ml[lane].x : -INFINITY);
+    const float mx = warp_max(lane < ns ? ml(lane).x : -INFINITY);
     a.sum(po, ml, ns, 0, 1, mx, lane);
-#pragma unroll
-    for (int e = 0; e < E; e++) out[row * D + E * lane + e] = f2bf(a.acc[e] / a.l);
+    a.write(out + row * D, lane);
     return;
   }
   if (kRows) return;
   float mx = -INFINITY;
-  for (int i = threadIdx.x; i < ns; i += kMergeWarps * 32) mx = fmaxf(mx, ml[i].x);
+  for (int i = threadIdx.x; i < ns; i += kMergeWarps * 32) mx = fmaxf(mx, ml(i).x);
   mx = warp_max(mx);
   if (lane == 0) smx[warp] = mx;
   __syncthreads();
@@ -579,7 +601,7 @@ cudaError_t launch_decode(const DecodeParams& p, int B, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
   e = launch_ex(decode_kernel<D, NG, BS>, dim3((p.max_splits + kDecWarps - 1) / kDecWarps, p.hkv * p.head_tiles, B),
                 dim3(kDecThreads), C::kSmem, stream, 0, p);
-  if (e != cudaSuccess || p.max_splits == 1) return e;
+  if (e != cudaSuccess || p.join) return e;
   const int64_t rows = (int64_t)B * p.hq;
   auto merge = [&](auto kernel, int64_t grid) {
     return launch_ex(kernel, dim3((unsigned)grid), dim3(kMergeWarps * 32), 0, stream, 0, (const float*)p.part_o,
@@ -590,6 +612,8 @@ cudaError_t launch_decode(const DecodeParams& p, int B, cudaStream_t stream) {
 }
 
 }  // namespace kv4
+
+bool kv4_decode_joins(int64_t max_splits) { return max_splits <= kv4::kDecWarps; }
 
 int64_t kv4_max_splits(int64_t max_len) {
   // the most of any length up to max_len: the count falls where the splits get longer
@@ -621,6 +645,7 @@ cudaError_t launch_kv4_decode(const Kv4DecodeArgs& a, cudaStream_t stream) {
   p.hkv = a.c.hkv;
   p.head_tiles = (a.hq / a.c.hkv + 7) / 8;
   p.max_splits = a.max_splits;
+  p.join = a.max_splits <= kv4::kDecWarps;
   p.scale_log2 = a.scale * kv4::kLog2eF;
   if ((int64_t)p.hkv * p.head_tiles > 65535 || (int64_t)a.B * a.hq > INT32_MAX) return cudaErrorInvalidValue;
   return kv4::pick(a.c.d, a.c.groups, a.c.block_size, [&](auto d, auto ng, auto bs) {

@@ -825,7 +825,7 @@ torch::Tensor paged_decode_kv4(torch::Tensor q, torch::Tensor cache, torch::Tens
   a.out = out.data_ptr();
   const int64_t splits = es::kv4_max_splits(max_model_len);
   a.max_splits = (int)splits;
-  if (splits > 1) {
+  if (!es::kv4_decode_joins(splits)) {
     part = torch::empty({B * hq * splits * (d + 2)}, q.options().dtype(at::kFloat));
     a.part_o = part.data_ptr<float>();
     a.part_ml = a.part_o + B * hq * splits * d;
