@@ -147,6 +147,18 @@ def test_decode_extremes(kops):
     held_to(out, want, mag, DECODE_MAG)
 
 
+@pytest.mark.parametrize("group", [64, 128])
+def test_decode_averages_of_long_histories(kops, group):
+    """What 50K keys of like weight average to is a hundredth of their codes' sum, so nothing may lean one
+    way. Over all values: bf16's rounding, 0.0017 of the norm, and the noise of P * scale in f16, 0.0005
+    (2^-12 / sqrt 3 of scale * code, 3.4 times the values' own deviation), at half as much again."""
+    hq, hkv, d, bs = 32, 8, 128, 16
+    q, cache, tables, ctx, last = batch([50001, 49000], [1, 1], hq, hkv, d, group, bs, 14)
+    out = kops.decode_attention_kv4(q, cache, tables, ctx, d**-0.5, bs)
+    want, _ = oracle(q, cache, tables, ctx, last, d**-0.5, bs)
+    assert float((out.double() - want).norm() / want.norm()) < 1.5 * (0.0017**2 + 0.0005**2) ** 0.5
+
+
 def test_decode_nan_stays_in_its_sequence(kops):
     hq, hkv, d, group, bs = 8, 2, 64, 64, 16
     q, cache, tables, ctx, last = batch([100, 100, 100], [1] * 3, hq, hkv, d, group, bs, 12)
