@@ -714,16 +714,28 @@ __global__ void __launch_bounds__(128) prefill_merge_kernel(PreParams p) {
   float acc[E], l = 0.f;
 #pragma unroll
   for (int e = 0; e < E; e++) acc[e] = 0.f;
+  const float* po = p.part_o + rh * p.max_splits * D + E * lane;  // a lane E neighbouring channels
+#pragma unroll 4
   for (int i = 0; i < ns; i++) {
-    const float mi = ml[2 * i];
-    const float f = mi == mx ? 1.f : ex2(mi - mx);
-    l = fmaf(ml[2 * i + 1], f, l);
-    const float* po = p.part_o + (rh * p.max_splits + i) * D;
+    const float2 t = reinterpret_cast<const float2*>(ml)[i];
+    const float f = t.x == mx ? 1.f : ex2(t.x - mx);
+    l = fmaf(t.y, f, l);
+    float v[E];
+    if (E == 4) {
+      const float4 x = *reinterpret_cast<const float4*>(po + (int64_t)i * D);
+      v[0] = x.x, v[1] = x.y, v[E - 2] = x.z, v[E - 1] = x.w;
+    } else {
+      const float2 x = *reinterpret_cast<const float2*>(po + (int64_t)i * D);
+      v[0] = x.x, v[1] = x.y;
+    }
 #pragma unroll
-    for (int e = 0; e < E; e++) acc[e] = fmaf(po[e * 32 + lane], f, acc[e]);
+    for (int e = 0; e < E; e++) acc[e] = fmaf(v[e], f, acc[e]);
   }
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;  // no visible key in any split: zeros
 #pragma unroll
-  for (int e = 0; e < E; e++) p.out[rh * D + e * 32 + lane] = f2bf(l > 0.f || l != l ? acc[e] / l : 0.f);
+  for (int e = 0; e < E; e += 2)
+    *reinterpret_cast<__nv_bfloat162*>(p.out + rh * D + E * lane + e) =
+        __floats2bfloat162_rn(inv == 0.f ? 0.f : acc[e] * inv, inv == 0.f ? 0.f : acc[e + 1] * inv);
 }
 
 template <int D, int NG, int BS>
