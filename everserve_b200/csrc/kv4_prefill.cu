@@ -528,23 +528,21 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
       __syncwarp();
       float cq;
       {
-        uint4 qv[U];
         __nv_bfloat162 mx = __floats2bfloat162_rn(0.f, 0.f);
-#pragma unroll
-        for (int k = 0; k < U; k++) qv[k] = *unit(r, k);
-#pragma unroll
+#pragma unroll 4
         for (int k = 0; k < U; k++) {
-          const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&qv[k]);
+          const uint4 qv = *unit(r, k);
+          const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&qv);
 #pragma unroll
           for (int e = 0; e < 4; e++) mx = __hmax2(mx, __habs2(h[e]));
         }
         const float2 m2 = __bfloat1622float2(mx);
         const int qe = pre_exponent(__float_as_uint(fmaxf(m2.x, m2.y)));
         const float qf = pre_pow2(kTop - qe);
-#pragma unroll
+#pragma unroll 2
         for (int k = 0; k < U; k++) {
           float f[8];
-          unpack8(qv[k], f);
+          unpack8(*unit(r, k), f);
           uint32_t h[4];
 #pragma unroll
           for (int x = 0; x < 4; x++) {
@@ -654,7 +652,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
       const float scale_o = ns > 1 ? unit_o : none ? 0.f : unit_o / l;
       const int64_t part = out_row / D * p.max_splits + it.split;
       if (ns == 1) {
-#pragma unroll
+#pragma unroll 1
         for (int q = 0; q < D / 32; q++) {
           uint32_t v[32];
           ptx::tmem_ld32(o_t + q * 32, v);
@@ -668,7 +666,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
           }
         }
         __syncwarp();
-#pragma unroll 8
+#pragma unroll 2
         for (int x = 0; x < U; x++) {
           const int rr = w0 + x * kPass + lane / U;
           const int64_t at = row_of(it, rr, (int64_t)p.hq * D);
