@@ -16,7 +16,8 @@
 //     memory, 128-byte swizzled, each freed by itself: K's by the second S, so that the next keys are there
 //     while this tile's softmax runs (one barrier for both: 711 us for the 8192-row prompt);
 //   * 12 issues the MMAs: S_t = Q_t . K_j^T and O_t += P_t . V_j for t = 0, 1 in turn, P read from TMEM;
-//   * 0-3 and 4-7 do the softmax of tiles 0 and 1, a thread a row: S from TMEM, P back over it in f16.
+//   * 0-3 and 4-7 do the softmax of tiles 0 and 1, a thread a row: S from TMEM, P back over it in f16, the
+//     first half of it for the tensor core to start on (P as a whole: 16 prompts 136 us instead of 131).
 // While one tile's softmax runs, the tensor core works for the other. The running maximum moves (and O in
 // TMEM is rescaled) only when a score passes it by 2^6, so most tiles leave O alone. A row's sums are fp32.
 // Registers go where they are needed: 184 a softmax thread (a row's 128 scores at once), 104 a converting one.
@@ -27,11 +28,13 @@
 // synchronisation; a warp of each CTA hands items out ahead of their readers. All waits are bounded and end in
 // the status word.
 //
-// Measured (32 / 8 heads of 128): one prompt of 8192 rows in 648 us, 848 TFLOP/s, half of what cuBLAS reaches.
-// A key tile takes 4,400 cycles where its 32 MMAs need 2,060 and its exponentials 2,050: each query tile's chain
-// S -> softmax (1,900) -> P -> MMAs is longer than the two tiles' overlap hides, and the conversion's stores
-// and the MMAs share the shared memory's bandwidth. 16 prompts of 8191 rows in all take 141 us: an item of three
-// key tiles pays as much again for its query, its first conversion and its output.
+// Measured (32 / 8 heads of 128): one prompt of 8192 rows in 622 us, 885 TFLOP/s, half of what cuBLAS reaches.
+// A key tile takes 4,300 cycles where its 32 MMAs need 2,060 and its exponentials 2,050: each query tile's chain
+// S -> softmax -> P -> MMAs is longer than the two tiles' overlap hides, and the conversion's stores and the MMAs
+// share the shared memory's bandwidth. (An eighth of the exponentials as polynomials on the FMA pipe: slower,
+// 654 us; instructions bound the softmax, not the exponential unit.) 16 prompts of 8191 rows in all take 119 us:
+// an item of three key tiles pays as much again for its query, its first conversion and its output. Two more
+// warps that copied the next item's query ahead made that 130 us.
 #include <atomic>
 
 #include "api.h"
@@ -53,6 +56,14 @@ static_assert(kSoftRegs * kSoftThreads + kConvRegs * kConvThreads + kMmaRegs * 1
               "the split draws on the registers of the launch, 128 a thread");
 constexpr int kTmem = 512;  // S0, S1 (128 columns each, P over them), O0, O1
 
+// Wait for phase `parity` of `bar`: at most 2^20 tries of up to 2 us each. (Reading the global timer for the bound
+// is more code at each of 16 places, which warps in different roles fetch at once: 122.4 us for 16 prompts.)
+ES_DEVICE bool wait_for(uint64_t* bar, uint32_t parity) {
+  for (uint32_t tries = 0; tries < (1u << 20); tries++)
+    if (ptx::mbar_try_wait(bar, parity, 2000u)) return true;
+  return false;
+}
+
 template <int D>
 struct PreCfg {
   static constexpr int kChunk = kRows * 128;           // one 64-channel chunk of a 128-row operand
@@ -62,6 +73,7 @@ struct PreCfg {
 
 constexpr float kPreSlack = 6.f;  // log2 of how far a score may pass the running maximum
 constexpr float kPreBits = 9.f;   // P enters f16 as at most 2^(6 + 9)
+constexpr int kFirst = 2;         // quarters of a tile's P that the tensor core takes while the rest is computed
 constexpr int kTop = 13;          // operands are scaled to below 2^(kTop + 1)
 
 template <int N>
@@ -107,6 +119,7 @@ struct Item {
 ES_DEVICE bool find_item(const PreParams& p, int bs, int idx, Item& it) {
   const int lane = threadIdx.x & 31;
   int before = 0;
+#pragma unroll 1
   for (int s0 = 0; s0 < p.S; s0 += 32) {
     const int s = s0 + lane;
     int rows = 0, r0 = 0, ctx = 0, tiles = 0, ns = 0, chunk = 1, items = 0;
@@ -124,12 +137,12 @@ ES_DEVICE bool find_item(const PreParams& p, int bs, int idx, Item& it) {
     int src = lane;
     if (p.S > 1) {
       int rank = 0;
-#pragma unroll 4
+#pragma unroll 1
       for (int k = 0; k < 32; k++) {
         const int c = __shfl_sync(0xffffffffu, ctx, k);
         rank += c > ctx || (c == ctx && k < lane);
       }
-#pragma unroll 4
+#pragma unroll 1
       for (int k = 0; k < 32; k++)
         if (__shfl_sync(0xffffffffu, rank, k) == lane) src = k;
       items = __shfl_sync(0xffffffffu, items, src);
@@ -150,11 +163,11 @@ ES_DEVICE bool find_item(const PreParams& p, int bs, int idx, Item& it) {
       it.row0 = __shfl_sync(0xffffffffu, r0, src);
       it.ctx = __shfl_sync(0xffffffffu, ctx, src);
       it.chunk = __shfl_sync(0xffffffffu, chunk, src);
-      const int t = __shfl_sync(0xffffffffu, tiles, src), per = __shfl_sync(0xffffffffu, ns, src) * p.hkv;
-      const int at = idx - first;
-      it.tile = t - 1 - at / per;
-      it.split = at % per / p.hkv;
-      it.head = at % per % p.hkv;
+      const int t = __shfl_sync(0xffffffffu, tiles, src), per = __shfl_sync(0xffffffffu, ns, src);
+      const uint32_t at = idx - first, group = at / (uint32_t)p.hkv, splits = (uint32_t)per;
+      it.tile = t - 1 - (int)(group / splits);
+      it.split = (int)(group % splits);
+      it.head = (int)(at - group * p.hkv);
       return true;
     }
     before += total;
@@ -273,7 +286,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
   uint64_t *k_full = bar + 8, *k_empty = bar + 10, *v_full = bar + 12, *v_empty = bar + 14;
   uint64_t* mma_done = bar + 16;
   uint64_t *item_full = bar + 17, *item_empty = bar + 19;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 21);
+  uint64_t* p_part = bar + 21;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 23);
   __shared__ int s_fail;
   __shared__ Item s_item[2];             // items ahead of their readers; seq -1: there is none
   __shared__ uint32_t s_bound[2][2][4];  // [tile parity][K, V][converting warp]: largest magnitudes' bits
@@ -287,6 +301,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
       ptx::mbar_init(&item_empty[i], 13);  // a lane of every warp that reads items
       ptx::mbar_init(&q_full[i], 128);
       ptx::mbar_init(&s_full[i], 1);
+      ptx::mbar_init(&p_part[i], 128);
       ptx::mbar_init(&p_full[i], 128);
       ptx::mbar_init(&o_full[i], 1);
       ptx::mbar_init(&k_full[i], kConvThreads);
@@ -311,7 +326,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
   uint32_t taken = 0;
   auto next_item = [&]() {
     const int s = taken & 1;
-    ok = __all_sync(0xffffffffu, ptx::mbar_wait(&item_full[s], (taken >> 1) & 1));
+    ok = __all_sync(0xffffffffu, wait_for(&item_full[s], (taken >> 1) & 1));
     if (!ok) return false;
     it = s_item[s];
     __syncwarp();
@@ -357,7 +372,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
         kb = __reduce_max_sync(0xffffffffu, kb);
         vb = __reduce_max_sync(0xffffffffu, vb);
         if (lane == 0) s_bound[s][0][warp - 8] = kb, s_bound[s][1][warp - 8] = vb;
-        if (n >= 2) ok = __all_sync(0xffffffffu, ptx::mbar_wait(&k_empty[s], ((n >> 1) - 1) & 1)) && ok;
+        if (n >= 2) ok = __all_sync(0xffffffffu, wait_for(&k_empty[s], ((n >> 1) - 1) & 1)) && ok;
         left = ptx::named_bar_or(1, kConvThreads, !ok);
         if (left) break;
         const uint32_t *bk = s_bound[s][0], *bv = s_bound[s][1];
@@ -375,7 +390,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
         }
         ptx::fence_proxy_async();
         ptx::mbar_arrive(&k_full[s]);
-        if (n >= 2) ok = __all_sync(0xffffffffu, ptx::mbar_wait(&v_empty[s], ((n >> 1) - 1) & 1));
+        if (n >= 2) ok = __all_sync(0xffffffffu, wait_for(&v_empty[s], ((n >> 1) - 1) & 1));
 #pragma unroll
         for (int i = 0; i < P; i++) {
           store_piece<D, NG>(kt + C::kTile, i * (kConvThreads / P) + tid / P, tid % P, vc[i], vm[i], vf);
@@ -400,7 +415,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
       for (uint32_t k = 0; ok; k++) {
         const bool any = find_item(p, BS, idx, it);
         if (any) span(p, it);
-        if (k >= 2) ok = __all_sync(0xffffffffu, ptx::mbar_wait(&item_empty[k & 1], ((k >> 1) - 1) & 1));
+        if (k >= 2) ok = __all_sync(0xffffffffu, wait_for(&item_empty[k & 1], ((k >> 1) - 1) & 1));
         if (!ok) break;
         if (lane == 0) {
           if (!any) it.seq = -1;
@@ -440,9 +455,9 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
     while (ok && next_item()) {
       const int j0 = it.j0, j1 = it.j1;
       if (j0 >= j1) continue;
-      ok = __all_sync(0xffffffffu, ptx::mbar_wait(&k_full[n & 1], (n >> 1) & 1));
+      ok = __all_sync(0xffffffffu, wait_for(&k_full[n & 1], (n >> 1) & 1));
       for (int t = 0; ok && t < 2; t++) {
-        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&q_full[t], items & 1));
+        ok = __all_sync(0xffffffffu, wait_for(&q_full[t], items & 1));
         if (!ok) break;
         ptx::tc_fence_after();
         qk(t, n & 1);
@@ -451,14 +466,24 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
         const int s = n & 1;
 #pragma unroll 1
         for (int t = 0; t < 2; t++) {
-          if (t == 0) ok = __all_sync(0xffffffffu, ptx::mbar_wait(&v_full[s], (n >> 1) & 1));
-          ok = ok && __all_sync(0xffffffffu, ptx::mbar_wait(&p_full[t], n & 1));
+          if (t == 0) ok = __all_sync(0xffffffffu, wait_for(&v_full[s], (n >> 1) & 1));
+          const uint64_t b = v_desc + s * kStageStep;
+          ok = ok && __all_sync(0xffffffffu, wait_for(&p_part[t], n & 1));
           if (!ok) break;
           ptx::tc_fence_after();
           if (leader) {
-            const uint64_t b = v_desc + s * kStageStep;
 #pragma unroll 1
-            for (int kk = 0; kk < kKeys / 16; kk++)
+            for (int kk = 0; kk < 2 * kFirst; kk++)
+              ptx::mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, b + kk * (16 * 128 >> 4), idesc_o,
+                              (j > j0 || kk > 0) ? 1u : 0u);
+          }
+          __syncwarp();
+          ok = __all_sync(0xffffffffu, wait_for(&p_full[t], n & 1));
+          if (!ok) break;
+          ptx::tc_fence_after();
+          if (leader) {
+#pragma unroll 1
+            for (int kk = 2 * kFirst; kk < kKeys / 16; kk++)
               ptx::mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, b + kk * (16 * 128 >> 4), idesc_o,
                               (j > j0 || kk > 0) ? 1u : 0u);
             if (t == 1) ptx::mma_commit(&v_empty[s]);
@@ -466,7 +491,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
           }
           __syncwarp();
           if (j + 1 < j1) {
-            if (t == 0) ok = __all_sync(0xffffffffu, ptx::mbar_wait(&k_full[s ^ 1], ((n + 1) >> 1) & 1));
+            if (t == 0) ok = __all_sync(0xffffffffu, wait_for(&k_full[s ^ 1], ((n + 1) >> 1) & 1));
             if (!ok) break;
             ptx::tc_fence_after();
             qk(t, s ^ 1);  // after P_t . V in the tensor core's order, which P_t's columns wait for
@@ -479,7 +504,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
     if (warp == 12) {
       if (leader) ptx::mma_commit(mma_done);
       __syncwarp();
-      ptx::mbar_wait(mma_done, 0);  // nothing of this CTA is in flight past here
+      wait_for(mma_done, 0);  // nothing of this CTA is in flight past here
     }
   } else {
     // ---- softmax --------------------------------------------------------------------------------
@@ -499,30 +524,28 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
     auto unit = [&](int x, int k) {
       return reinterpret_cast<uint4*>(rows_s + (k >> 3) * C::kChunk + x * 128 + (((k & 7) ^ (x & 7)) << 4));
     };
-    // where row x of an item's tile is in memory (elements of q, of the output), or -1 past the sequence
-    auto row_of = [&](const Item& i, int x, int64_t stride) -> int64_t {
-      const int tk = (x * inv_g) >> 16, hh = x - tk * p.G;
-      const int at = i.tile * 2 * p.tt + t * p.tt + tk;
-      return tk < p.tt && at < i.rows ? (int64_t)(i.row0 + at) * stride + (i.head * p.G + hh) * D : -1;
-    };
     uint32_t n = 0, items = 0;
     while (ok && next_item()) {
       const int j0 = it.j0, j1 = it.j1, ns = it.ns;
-      const int64_t out_row = row_of(it, r, (int64_t)p.hq * D);  // -1: no row
       const int at = it.tile * 2 * p.tt + t * p.tt + token;
+      const bool real = token < p.tt && at < it.rows;
+      // where this thread's row is in memory: its elements of the query (-1: no row), its row of the output. The
+      // lanes that move another's row ask it: a row of G heads takes a division and 64-bit products to find.
+      const int64_t q_at = real ? (int64_t)(it.row0 + at) * p.q_stride + (it.head * p.G + head) * D : -1;
+      const int64_t out_row = real ? (int64_t)(it.row0 + at) * p.hq + it.head * p.G + head : -1;
       const int pos = it.ctx - it.rows + at;
-      if (out_row >= 0 && it.split == 0 && it.head == 0 && head == 0 && p.part_ns != nullptr) p.part_ns[it.row0 + at] = ns;
+      if (real && it.split == 0 && it.head == 0 && head == 0 && p.part_ns != nullptr) p.part_ns[it.row0 + at] = ns;
       if (j0 >= j1) {
-        if (it.split == 0 && out_row >= 0)  // no key at all
-          for (int i = 0; i < U; i++) reinterpret_cast<uint4*>(p.out + out_row)[i] = make_uint4(0, 0, 0, 0);
+        if (it.split == 0 && real)  // no key at all
+          for (int i = 0; i < U; i++) reinterpret_cast<uint4*>(p.out + out_row * D)[i] = make_uint4(0, 0, 0, 0);
         continue;
       }
       // the query: asynchronous copies in memory's order, then each thread scales its own row by a power of two
 #pragma unroll 4
       for (int x = 0; x < U; x++) {
-        const int rr = w0 + x * kPass + lane / U;
-        const int64_t at = row_of(it, rr, p.q_stride);
-        ptx::cp_async16(unit(rr, lane % U), p.q + max(at, (int64_t)0) + 8 * (lane % U), at >= 0);
+        const int from = x * kPass + lane / U;
+        const int64_t at = __shfl_sync(0xffffffffu, q_at, from);
+        ptx::cp_async16(unit(w0 + from, lane % U), p.q + max(at, (int64_t)0) + 8 * (lane % U), at >= 0);
       }
       ptx::cp_async_wait_all();
       __syncwarp();
@@ -560,7 +583,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
       float m = -INFINITY, l = 0.f;
       int vrun = -100;
       for (int j = j0; j < j1; j++, n++) {
-        ok = __all_sync(0xffffffffu, ptx::mbar_wait(&s_full[t], n & 1));
+        ok = __all_sync(0xffffffffu, wait_for(&s_full[t], n & 1));
         if (!ok) break;
         ptx::tc_fence_after();
         const float c = cq * pre_pow2(s_exp[n & 3][0] - kTop);
@@ -572,48 +595,25 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
         const int key0 = j * kKeys;
         if (__any_sync(0xffffffffu, key0 + kKeys - 1 > pos)) {
 #pragma unroll
-          for (int i = 0; i < 128; i++)
-            if (key0 + i > pos) v[i] = 0xFF800000u;  // -infinity
-        }
-        if (j == j0) {  // the first keys: their maximum, and nothing to rescale
-          float mx[4];
-#pragma unroll
-          for (int q = 0; q < 4; q++) mx[q] = __uint_as_float(v[q]);
-#pragma unroll
-          for (int i = 4; i < 128; i++) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(v[i]));
-          m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
-          vrun = ve;
-        }
-        // P times 2^(kPreBits + ve - vrun), back over the columns of S; the row's sum and the tile's maximum
-        float mx[4];
-        uint64_t sum[2];
-        const uint64_t cc = ptx::pair_f32(c, c);
-        auto soft = [&](float add) {
-          const float mc = (m == -INFINITY ? 0.f : -m) + add;
-          const uint64_t mm = ptx::pair_f32(mc, mc);
-          sum[0] = sum[1] = ptx::pair_f32(0.f, 0.f);
-#pragma unroll
-          for (int q = 0; q < 4; q++) mx[q] = -INFINITY;
-#pragma unroll
           for (int q = 0; q < 4; q++) {
-            uint32_t pk[16];
+            const int seen = max(0, min(32, pos + 1 - key0 - 32 * q));  // of these 32 keys
+            const uint32_t hide = seen < 32 ? 0xFFFFFFFFu << seen : 0u;
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-              const float x = __uint_as_float(v[q * 32 + 2 * i]), y = __uint_as_float(v[q * 32 + 2 * i + 1]);
-              const float2 e = ptx::unpair_f32(ptx::fma_f32x2(ptx::pair_f32(x, y), cc, mm));
-              const float a = ex2(e.x), b = ex2(e.y);
-              mx[i & 3] = fmaxf(fmaxf(mx[i & 3], x), y);
-              sum[i & 1] = ptx::add_f32x2(sum[i & 1], ptx::pair_f32(a, b));
-              const __half2 h = __floats2half2_rn(a, b);
-              pk[i] = *reinterpret_cast<const uint32_t*>(&h);
-            }
-            ptx::tmem_st16(s_t + q * 16, pk);
+            for (int i = 0; i < 32; i++)
+              if (hide & (1u << i)) v[32 * q + i] = 0xFF800000u;  // -infinity
           }
-        };
-        // against the maximum so far, which holds for all but a few tiles: the tile's own is known in passing
-        soft(kPreBits + (float)(ve - vrun));
+        }
+        float mx[4];
+#pragma unroll
+        for (int q = 0; q < 4; q++) mx[q] = __uint_as_float(v[q]);
+#pragma unroll
+        for (int i = 4; i < 128; i += 8)
+#pragma unroll
+          for (int q = 0; q < 4; q++)
+            mx[q] = i + 4 < 128 ? fmaxf(fmaxf(mx[q], __uint_as_float(v[i + q])), __uint_as_float(v[min(i + 4 + q, 127)]))
+                                : fmaxf(mx[q], __uint_as_float(v[i + q]));
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
-        if (__any_sync(0xffffffffu, top > m + kPreSlack || ve > vrun)) {
+        if (__any_sync(0xffffffffu, j == j0 || top > m + kPreSlack || ve > vrun)) {
           const float mn = fmaxf(m, top);
           const float a = m == -INFINITY ? 0.f : ex2(m - mn);
           const int vn = max(vrun, ve);
@@ -632,16 +632,39 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
             }
           }
           vrun = vn;
-          soft(kPreBits + (float)(ve - vrun));
         }
+        // P times 2^(kPreBits + ve - vrun), back over the columns of S, and the row's sum
         const float add = kPreBits + (float)(ve - vrun);
+        const float mc = (m == -INFINITY ? 0.f : -m) + add;
+        const uint64_t cc = ptx::pair_f32(c, c), mm = ptx::pair_f32(mc, mc);
+        uint64_t sum[2];
+        sum[0] = sum[1] = ptx::pair_f32(0.f, 0.f);
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            const float x = __uint_as_float(v[q * 32 + 2 * i]), y = __uint_as_float(v[q * 32 + 2 * i + 1]);
+            const float2 e = ptx::unpair_f32(ptx::fma_f32x2(ptx::pair_f32(x, y), cc, mm));
+            const float a = ex2(e.x), b = ex2(e.y);
+            sum[i & 1] = ptx::add_f32x2(sum[i & 1], ptx::pair_f32(a, b));
+            const __half2 h = __floats2half2_rn(a, b);
+            pk[i] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+          ptx::tmem_st16(s_t + q * 16, pk);
+          if (q + 1 == kFirst) {
+            ptx::tmem_wait_st();
+            ptx::tc_fence_before();
+            ptx::mbar_arrive(&p_part[t]);
+          }
+        }
         ptx::tmem_wait_st();
         ptx::tc_fence_before();
         ptx::mbar_arrive(&p_full[t]);
         const float2 both = ptx::unpair_f32(ptx::add_f32x2(sum[0], sum[1]));
         l = fmaf(both.x + both.y, ex2(-add), l);
       }
-      if (ok) ok = __all_sync(0xffffffffu, ptx::mbar_wait(&o_full[t], items & 1));
+      if (ok) ok = __all_sync(0xffffffffu, wait_for(&o_full[t], items & 1));
       if (!ok) break;
       items++;
       ptx::tc_fence_after();
@@ -650,7 +673,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
       const float unit_o = pre_pow2(vrun - kTop - (int)kPreBits);
       const bool none = !(l > 0.f || l != l);  // no visible key: zeros
       const float scale_o = ns > 1 ? unit_o : none ? 0.f : unit_o / l;
-      const int64_t part = out_row / D * p.max_splits + it.split;
+      const int64_t part = out_row * p.max_splits + it.split;
       if (ns == 1) {
 #pragma unroll 1
         for (int q = 0; q < D / 32; q++) {
@@ -666,12 +689,12 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
           }
         }
         __syncwarp();
-#pragma unroll 2
+#pragma unroll 4
         for (int x = 0; x < U; x++) {
-          const int rr = w0 + x * kPass + lane / U;
-          const int64_t at = row_of(it, rr, (int64_t)p.hq * D);
-          const uint4 y = *unit(rr, lane % U);
-          if (at >= 0) reinterpret_cast<uint4*>(p.out + at)[lane % U] = y;
+          const int from = x * kPass + lane / U;
+          const int64_t at = __shfl_sync(0xffffffffu, out_row, from);
+          const uint4 y = *unit(w0 + from, lane % U);
+          if (at >= 0) reinterpret_cast<uint4*>(p.out + at * D)[lane % U] = y;
         }
         __syncwarp();
       } else {
@@ -680,7 +703,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
           uint32_t v[32];
           ptx::tmem_ld32(o_t + q * 32, v);
           ptx::tmem_wait_ld();
-          if (out_row < 0) continue;
+          if (!real) continue;
 #pragma unroll
           for (int u = 0; u < 8; u++) {
             float4 f;
@@ -690,7 +713,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
           }
         }
       }
-      if (out_row >= 0 && ns > 1) p.part_ml[2 * part] = m, p.part_ml[2 * part + 1] = l;
+      if (real && ns > 1) p.part_ml[2 * part] = m, p.part_ml[2 * part + 1] = l;
       ptx::tc_fence_before();
     }
     if (!ok) s_fail = 1;

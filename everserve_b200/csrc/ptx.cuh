@@ -44,6 +44,19 @@ ES_DEVICE bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 
+// The same, suspended for `hint_ns` at most.
+ES_DEVICE bool mbar_try_wait(uint64_t* bar, uint32_t parity, uint32_t hint_ns) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(hint_ns)
+      : "memory");
+  return ok != 0;
+}
+
 // Whether phase `parity` of `bar` has completed, without waiting (mbarrier.test_wait).
 ES_DEVICE bool mbar_test(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
