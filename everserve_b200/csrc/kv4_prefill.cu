@@ -669,7 +669,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
       items++;
       ptx::tc_fence_after();
       // the output: through this warp's rows of the query tile (read by no MMA any more), so that a store
-      // covers whole rows; a split's in fp32, each thread its row
+      // covers whole rows; a split's in fp32, 32 channels at a time (a thread its own row straight to memory, 32 lines
+      // an instruction: 113 instead of 105 us for 509 rows on 0-40K keys)
       const float unit_o = pre_pow2(vrun - kTop - (int)kPreBits);
       const bool none = !(l > 0.f || l != l);  // no visible key: zeros
       const float scale_o = ns > 1 ? unit_o : none ? 0.f : unit_o / l;
@@ -703,14 +704,25 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
           uint32_t v[32];
           ptx::tmem_ld32(o_t + q * 32, v);
           ptx::tmem_wait_ld();
-          if (!real) continue;
+          auto cell = [&](int x, int k) {  // 16-byte unit k of row x, 128 bytes a row
+            return reinterpret_cast<float4*>(rows_s + x * 128 + ((k ^ (x & 7)) << 4));
+          };
 #pragma unroll
           for (int u = 0; u < 8; u++) {
             float4 f;
             f.x = __uint_as_float(v[4 * u]) * scale_o, f.y = __uint_as_float(v[4 * u + 1]) * scale_o;
             f.z = __uint_as_float(v[4 * u + 2]) * scale_o, f.w = __uint_as_float(v[4 * u + 3]) * scale_o;
-            reinterpret_cast<float4*>(p.part_o + part * D)[q * 8 + u] = f;
+            *cell(r, u) = f;
           }
+          __syncwarp();
+#pragma unroll 4
+          for (int x = 0; x < 8; x++) {
+            const int from = x * 4 + lane / 8;
+            const int64_t to = __shfl_sync(0xffffffffu, real ? part : -1, from);
+            const float4 y = *cell(w0 + from, lane & 7);
+            if (to >= 0) reinterpret_cast<float4*>(p.part_o + to * D + q * 32)[lane & 7] = y;
+          }
+          __syncwarp();
         }
       }
       if (real && ns > 1) p.part_ml[2 * part] = m, p.part_ml[2 * part + 1] = l;
