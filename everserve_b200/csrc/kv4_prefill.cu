@@ -28,7 +28,8 @@
 // synchronisation; a warp of each CTA hands items out ahead of their readers. All waits are bounded and end in
 // the status word.
 //
-// Measured (32 / 8 heads of 128): one prompt of 8192 rows in 622 us, 885 TFLOP/s, half of what cuBLAS reaches.
+// Measured (32 / 8 heads of 128): one prompt of 8192 rows in 622-633 us, 870-885 TFLOP/s, half of what cuBLAS
+// reaches.
 // A key tile takes 4,300 cycles where its 32 MMAs need 2,060 and its exponentials 2,050: each query tile's chain
 // S -> softmax -> P -> MMAs is longer than the two tiles' overlap hides, and the conversion's stores and the MMAs
 // share the shared memory's bandwidth. (An eighth of the exponentials as polynomials on the FMA pipe: slower,
