@@ -37,6 +37,7 @@
 // an item of three key tiles pays as much again for its query, its first conversion and its output. Two more
 // warps that copied the next item's query ahead made that 130 us.
 #include <atomic>
+#include <climits>
 
 #include "api.h"
 #include "common.cuh"
@@ -249,10 +250,13 @@ struct Source {
   }
 };
 
-// The bits of a bound on a group's magnitudes.
+// The bits of a bound on a group's magnitudes; kNotFinite or more for a group that reads as NaN.
+constexpr uint32_t kNotFinite = 0x7F800000u;
 ES_DEVICE uint32_t bound_of(uint32_t pair) {
   const float z = pair_zero(pair);
-  return __float_as_uint(fmaxf(fabsf(z), fabsf(fmaf(15.f, pair_scale(pair), z))));
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(fabsf(z)), "f"(fabsf(fmaf(15.f, pair_scale(pair), z))));
+  return __float_as_uint(d);
 }
 
 // One piece of row `row` into a tile's swizzled layout, times f.
@@ -293,6 +297,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
   __shared__ Item s_item[2];             // items ahead of their readers; seq -1: there is none
   __shared__ uint32_t s_bound[2][2][4];  // [tile parity][K, V][converting warp]: largest magnitudes' bits
   __shared__ int s_exp[4][2];            // [tile & 3][K, V]: the tile's exponents
+  __shared__ int s_nan[4][NG];           // [item & 3][group]: the item's first key whose V reads as NaN
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -340,8 +345,9 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
     regs_down<kConvRegs>();
     constexpr int P = D / 32;
     const int tid = threadIdx.x - kSoftThreads;
-    uint32_t n = 0;  // key tiles converted so far, over all items
+    uint32_t n = 0, items = 0;  // key tiles converted so far, over all items; items with any
     bool left = false;
+    if (tid < NG) s_nan[0][tid] = INT_MAX;
     while (!left) {
       const bool any = next_item();
       left = ptx::named_bar_or(1, kConvThreads, !ok);  // where a wait of one of the converting warps ran out, all leave
@@ -372,14 +378,37 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
           for (int g = 0; g < NG; g++) kb = max(kb, bound_of(km[i][g])), vb = max(vb, bound_of(vm[i][g]));
         kb = __reduce_max_sync(0xffffffffu, kb);
         vb = __reduce_max_sync(0xffffffffu, vb);
+        if (__builtin_expect(max(kb, vb) >= kNotFinite, 0)) {
+          // A group that reads as NaN sets no exponent. K's stays in its key's scores, which a mask replaces; V's
+          // would reach every row of the tile through a probability of zero, so it counts as zero here, and the
+          // rows that see its key, or a later one, get their NaN in the end.
+          kb = vb = 0;
+#pragma unroll
+          for (int i = 0; i < P; i++)
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+              const uint32_t k = bound_of(km[i][g]), v = bound_of(vm[i][g]);
+              if (k < kNotFinite) kb = max(kb, k);
+              if (v < kNotFinite) {
+                vb = max(vb, v);
+              } else {
+                vm[i][g] = 0;
+                atomicMin(&s_nan[items & 3][g], src.key(j, i));
+              }
+            }
+          kb = __reduce_max_sync(0xffffffffu, kb);
+          vb = __reduce_max_sync(0xffffffffu, vb);
+        }
         if (lane == 0) s_bound[s][0][warp - 8] = kb, s_bound[s][1][warp - 8] = vb;
         if (n >= 2) ok = __all_sync(0xffffffffu, wait_for(&k_empty[s], ((n >> 1) - 1) & 1)) && ok;
         left = ptx::named_bar_or(1, kConvThreads, !ok);
         if (left) break;
         const uint32_t *bk = s_bound[s][0], *bv = s_bound[s][1];
-        const int ke = pre_exponent(max(max(bk[0], bk[1]), max(bk[2], bk[3])));
+        kb = max(max(bk[0], bk[1]), max(bk[2], bk[3]));
+        vb = max(max(bv[0], bv[1]), max(bv[2], bv[3]));
+        const int ke = pre_exponent(kb);
         // (not far below the largest: a tile of small values leaves its probabilities' range alone)
-        const int ve = max(pre_exponent(max(max(bv[0], bv[1]), max(bv[2], bv[3]))), vr - 20);
+        const int ve = max(pre_exponent(vb), vr - 20);
         vr = max(vr, ve);
         if (tid == 0) s_exp[n & 3][0] = ke, s_exp[n & 3][1] = ve;
         const float kf = pre_pow2(kTop - ke), vf = pre_pow2(kTop - ve);
@@ -403,6 +432,10 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
         ptx::fence_proxy_async();
         ptx::mbar_arrive(&v_full[s]);
       }
+      // (the next entry, before the barrier ahead of its item: its last readers were the rows of the item three
+      // before this one, and the query of the item after that has been asked for since)
+      items++;
+      if (tid < NG) s_nan[items & 3][tid] = INT_MAX;
       if (src.bad && p.status) atomicExch(p.status, (int)kBadShape);
     }
     if (!ok) s_fail = 1;
@@ -667,6 +700,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
       }
       if (ok) ok = __all_sync(0xffffffffu, wait_for(&o_full[t], items & 1));
       if (!ok) break;
+      // (read here: ahead of the wait it costs 1,000 cycles an item, 16 prompts 125 us)
+      const bool hole0 = pos >= s_nan[items & 3][0], hole1 = pos >= s_nan[items & 3][NG - 1];
       items++;
       ptx::tc_fence_after();
       // the output: through this warp's rows of the query tile (read by no MMA any more), so that a store
@@ -675,6 +710,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
       const float unit_o = pre_pow2(vrun - kTop - (int)kPreBits);
       const bool none = !(l > 0.f || l != l);  // no visible key: zeros
       const float scale_o = ns > 1 ? unit_o : none ? 0.f : unit_o / l;
+      // a row that sees a V of NaN, by halves of the channels
+      const float scale0 = hole0 ? NAN : scale_o, scale1 = hole1 ? NAN : scale_o;
       const int64_t part = out_row * p.max_splits + it.split;
       if (ns == 1) {
 #pragma unroll 1
@@ -686,7 +723,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
           for (int u = 0; u < 4; u++) {
             float f[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) f[i] = none ? 0.f : __uint_as_float(v[u * 8 + i]) * scale_o;
+            for (int i = 0; i < 8; i++) f[i] = none ? 0.f : __uint_as_float(v[u * 8 + i]) * (q < D / 64 ? scale0 : scale1);
             *unit(r, q * 4 + u) = pack8(f);
           }
         }
@@ -705,14 +742,15 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
           uint32_t v[32];
           ptx::tmem_ld32(o_t + q * 32, v);
           ptx::tmem_wait_ld();
+          const float scale_q = q < D / 64 ? scale0 : scale1;
           auto cell = [&](int x, int k) {  // 16-byte unit k of row x, 128 bytes a row
             return reinterpret_cast<float4*>(rows_s + x * 128 + ((k ^ (x & 7)) << 4));
           };
 #pragma unroll
           for (int u = 0; u < 8; u++) {
             float4 f;
-            f.x = __uint_as_float(v[4 * u]) * scale_o, f.y = __uint_as_float(v[4 * u + 1]) * scale_o;
-            f.z = __uint_as_float(v[4 * u + 2]) * scale_o, f.w = __uint_as_float(v[4 * u + 3]) * scale_o;
+            f.x = __uint_as_float(v[4 * u]) * scale_q, f.y = __uint_as_float(v[4 * u + 1]) * scale_q;
+            f.z = __uint_as_float(v[4 * u + 2]) * scale_q, f.w = __uint_as_float(v[4 * u + 3]) * scale_q;
             *cell(r, u) = f;
           }
           __syncwarp();

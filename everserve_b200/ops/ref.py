@@ -241,7 +241,11 @@ def kv4_attention(q, cache, block_tables, ctx_lens, last_rows, scale: float, blo
             score = torch.einsum("thd,nhd->htn", q[r0:r1].float(), k) * scale
             pos = torch.arange(n - (r1 - r0), n, device=q.device)
             score = score.masked_fill((torch.arange(n, device=q.device)[None] > pos[:, None])[None], float("-inf"))
-            o = torch.einsum("htn,nhd->thd", torch.softmax(score, -1), v)
+            bad = ~torch.isfinite(v)  # reaches the rows that see it alone, not the others times zero
+            o = torch.einsum("htn,nhd->thd", torch.softmax(score, -1), v.masked_fill(bad, 0.0))
+            if bool(bad.any()):
+                seen = (torch.arange(n, device=q.device)[None] <= pos[:, None]).float()
+                o = o.masked_fill(torch.einsum("tn,nhd->thd", seen, bad.float()) > 0, math.nan)
             out[r0:r1] = torch.where((pos >= 0)[:, None, None], o, torch.zeros_like(o)).to(q.dtype)
         r0 = r1
     return out

@@ -93,3 +93,24 @@ def test_copy_pages_pairs():
     for bad in ([[0, 1], [2, 1]], [[0, 1], [1, 2]], [[2, 2]]):
         with pytest.raises(ValueError):
             ops.copy_pages([cache], torch.tensor(bad))
+
+
+def test_not_finite_values_reach_the_rows_that_see_them():
+    """A group of V that reads as NaN makes its channels of the rows that see the key NaN, and no other."""
+    d, bs, n = 128, 16, 20
+    g = torch.Generator().manual_seed(4)
+    cache = torch.zeros(ref.kv4_cache_shape(2, 1, bs, d), dtype=torch.uint8)
+    qkv = torch.randn(n, 4 * d, generator=g)
+    tables, ctx, last = torch.tensor([[0, 1]], dtype=torch.int32), torch.tensor([n], dtype=torch.int32), torch.tensor([n - 1])
+
+    def attend():
+        at = torch.arange(n)
+        q = ref.rope_kv4_write(qkv, None, at, ref.cos_sin_table(d, 32, 1e4), at, cache, 2, 1, bs)
+        return ref.kv4_attention(q, cache, tables, ctx, last, 0.1, bs)
+
+    want = attend()
+    qkv[17, -1] = math.inf  # V's second group
+    got = attend()
+    bad = torch.zeros(n, 2, d, dtype=torch.bool)
+    bad[17:, :, 64:] = True
+    assert torch.equal(got.isnan(), bad) and torch.equal(got[~bad], want[~bad])
