@@ -289,7 +289,7 @@ int64_t kv4_max_splits(int64_t max_len);
 bool kv4_decode_joins(int64_t max_splits);  // the kernel joins that many itself: no scratch
 cudaError_t launch_kv4_decode(const Kv4DecodeArgs& a, cudaStream_t s);
 // prefill: causal attention of T new rows of S sequences; sequence s owns the rows up to last_rows[s], the
-// last of them at position ctx_lens[s] - 1
+// last of them at position ctx_lens[s] - 1; the rows past the last sequence's are zeroed
 struct Kv4PrefillArgs {
   Kv4Cache c;
   const void* q;  // [T, hq, d] rows of q_stride elements

@@ -52,7 +52,7 @@ constexpr int kRows = 128;  // rows of a tile (MMA M)
 constexpr int kKeys = 128;  // keys of a tile (MMA N of S, K of P.V)
 constexpr int kSoftThreads = 256;
 constexpr int kConvThreads = 128;
-constexpr int kPreThreads = kSoftThreads + kConvThreads + 128;  // (the MMA warp's group has three idle warps)
+constexpr int kPreThreads = kSoftThreads + kConvThreads + 128;  // (the MMA warp's group: kMmaRegs)
 constexpr int kSoftRegs = 184, kConvRegs = 104, kMmaRegs = 40;
 static_assert(kSoftRegs * kSoftThreads + kConvRegs * kConvThreads + kMmaRegs * 128 <= 128 * kPreThreads,
               "the split draws on the registers of the launch, 128 a thread");
@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
     }
     if (!ok) s_fail = 1;
   } else if (warp >= 12) {
-    // ---- MMA issuer, and the warp that hands out items (the group's other two idle) -----------------
+    // ---- MMA issuer, the warp that hands out items, and two that zero the rows of no sequence ---------
     regs_down<kMmaRegs>();
     if (warp == 13) {
       // An item's cost goes with its keys, so CTAs take their next one when they are ready for it, from one
@@ -459,6 +459,14 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
         if (!any) break;
         if (lane == 0) idx = (int)(gridDim.x + atomicAdd(p.next, 1u));
         idx = __shfl_sync(0xffffffffu, idx, 0);
+      }
+    }
+    if (warp >= 14) {
+      const int vecs = p.hq * (D / 8);
+      for (int64_t x = max((int64_t)0, p.last_rows[p.S - 1] + 1) + blockIdx.x; x < p.T; x += gridDim.x) {
+        uint4* row = reinterpret_cast<uint4*>(p.out) + x * vecs;
+        for (int i = threadIdx.x & 63; i < vecs; i += 64) row[i] = make_uint4(0, 0, 0, 0);
+        if ((threadIdx.x & 63) == 0 && p.part_ns != nullptr) p.part_ns[x] = 1;
       }
     }
     const bool failed = !ok;
@@ -842,7 +850,8 @@ int64_t kv4_prefill_splits(int64_t T, int64_t S, int64_t hq, int64_t hkv, int64_
 }
 
 cudaError_t launch_kv4_prefill(const Kv4PrefillArgs& a, cudaStream_t stream) {
-  if (a.T == 0 || a.S == 0) return cudaSuccess;
+  if (a.T == 0) return cudaSuccess;
+  if (a.S == 0) return cudaMemsetAsync(a.out, 0, (size_t)a.T * a.hq * a.c.d * sizeof(__nv_bfloat16), stream);
   if (a.c.hkv <= 0 || a.hq % a.c.hkv != 0 || a.hq / a.c.hkv > kv4::kRows || a.max_splits < 1 || !(a.scale > 0.f))
     return cudaErrorInvalidValue;
   if (a.c.s_block >> 4 > UINT32_MAX) return cudaErrorInvalidValue;

@@ -290,7 +290,7 @@ class KernelOps:
         """Causal attention of a step's new rows over their sequences' history in 4 bits (the rows' own
         keys and values written before): sequence s owns the rows up to last_rows[s] (int64, on the
         device), the last of them at position ctx_lens[s] - 1. q [T, hq, d] -> [T, hq, d]; a row without a
-        visible key gives zeros. `max_context` bounds the step's context lengths (default: what
+        visible key, or past the last sequence's, gives zeros. `max_context` bounds the step's context lengths (default: what
         block_tables can hold); it sizes the call's own workspace, nothing else."""
         if max_context is None:
             max_context = block_tables.shape[1] * block_size

@@ -90,3 +90,16 @@ def test_not_finite_reaches_the_rows_that_see_it(kops, hq, hkv, d, group, bs):
     for p in (kp, vp):
         p.nan_to_num_(1.0, 1.0, 1.0)
     assert bool(torch.isfinite(kops.prefill_attention_kv4(q, cache, tables, ctx, last, scale, bs)).all())
+
+
+def test_rows_of_no_sequence_are_zero(kops):
+    """Rows past the last sequence's, whatever the output's memory held."""
+    hq, hkv, d, group, bs = 8, 2, 128, 64, 16
+    q, cache, tables, ctx, last = batch([200, 5020], [100, 20], hq, hkv, d, group, bs, 42)
+    want = kops.prefill_attention_kv4(q, cache, tables, ctx, last, 0.1, bs)
+    more = torch.cat([q, torch.ones(77, hq, d, device="cuda").bfloat16()])
+    for seqs, rows in ((2, 120), (1, 100), (0, 0)):
+        torch.full((64 << 20,), math.nan, device="cuda")  # what the allocator hands out next
+        out = kops.prefill_attention_kv4(more, cache, tables, ctx, last[:seqs], 0.1, bs)
+        assert torch.equal(out[:rows], want[:rows]) and not bool(out[rows:].any())
+    assert kops.check_status() == 0
