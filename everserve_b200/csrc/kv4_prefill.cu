@@ -716,7 +716,9 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
       // covers whole rows; a split's in fp32, 32 channels at a time (a thread its own row straight to memory, 32 lines
       // an instruction: 113 instead of 105 us for 509 rows on 0-40K keys)
       const float unit_o = pre_pow2(vrun - kTop - (int)kPreBits);
-      const bool none = !(l > 0.f || l != l);  // no visible key: zeros
+      // no visible key: zeros; keys whose scores are all -infinity: NaN
+      const bool none = l == 0.f && pos < j0 * kKeys;
+      l = l == 0.f && !none ? NAN : l;
       const float scale_o = ns > 1 ? unit_o : none ? 0.f : unit_o / l;
       // a row that sees a V of NaN, by halves of the channels
       const float scale0 = hole0 ? NAN : scale_o, scale1 = hole1 ? NAN : scale_o;

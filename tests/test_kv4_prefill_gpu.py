@@ -103,3 +103,17 @@ def test_rows_of_no_sequence_are_zero(kops):
         out = kops.prefill_attention_kv4(more, cache, tables, ctx, last[:seqs], 0.1, bs)
         assert torch.equal(out[:rows], want[:rows]) and not bool(out[rows:].any())
     assert kops.check_status() == 0
+
+
+def test_visible_scores_of_minus_infinity(kops):
+    """A query whose scores all come to -infinity has NaN as its softmax, not the zeros of a row without keys."""
+    hq, hkv, d, group, bs = 2, 1, 64, 64, 16
+    q, cache, tables, ctx, last = batch([1, 3000], [1, 3], hq, hkv, d, group, bs, 43)
+    kp, _ = pairs_of(cache, d, bs)
+    kp[..., 1] = -100.0  # every channel of every key below zero
+    kp[..., 0] = 1.0
+    q = q.abs()
+    q[:, 0, 5] = math.inf
+    out = kops.prefill_attention_kv4(q, cache, tables, ctx, last, 0.1, bs)
+    assert bool(out[:, 0].isnan().all()) and bool(torch.isfinite(out[:, 1]).all())
+    assert kops.check_status() == 0
