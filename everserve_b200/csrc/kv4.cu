@@ -80,9 +80,9 @@ __global__ void __launch_bounds__(kThreads, 4) write_kernel(WriteParams p) {
   int64_t pos = p.positions[t];
   const int64_t slot = p.slots[t];
   bool bad = slot >= p.num_slots;
-  if (pos < 0 || pos >= p.max_pos) bad = true, pos = 0;  // no table row: reported, and rotated as position 0
+  if (pos < 0 || pos >= p.max_pos) bad = true, pos = 0;  // no table row: q is rotated as position 0
   if (bad && lane == 0 && p.status) atomicExch(p.status, (int)kBadShape);
-  const bool kept = slot >= 0 && slot < p.num_slots;
+  const bool kept = slot >= 0 && !bad;
   float c[8], s[8];
   {
     const float4* cs = reinterpret_cast<const float4*>(p.cos_sin + pos * D + 8 * l);

@@ -270,8 +270,8 @@ class KernelOps:
     # ---- the paged cache held in 4 bits (format: ref.kv4_cache_shape and above) -------------------
     def rope_kv4_write(self, qkv, bias, positions, cos_sin, slots, cache, hq, hkv, block_size):
         """RoPE on q and k, k and v quantised to 4 bits into their slots of `cache` (uint8, of
-        ``ref.kv4_cache_shape``); returns q [T, hq, d]. A negative slot is not written; a position or
-        slot out of range is reported by ``check_status``."""
+        ``ref.kv4_cache_shape``); returns q [T, hq, d]. A negative slot is not written; a row whose
+        position or slot is out of range is not written either, and reported by ``check_status``."""
         return self.C.rope_kv4_write(qkv, bias, positions, cos_sin, slots, cache, hq, hkv, block_size, self.status)
 
     def kv4_read(self, cache, slots, head_dim, block_size):
