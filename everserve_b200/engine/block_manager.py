@@ -26,6 +26,11 @@ class BlockManager:
     def free_blocks(self) -> int:
         return len(self._free)
 
+    @property
+    def shared_blocks(self) -> int:
+        """Blocks that more than one request holds."""
+        return len(self._shared)
+
     def blocks_for(self, num_tokens: int) -> int:
         return (num_tokens + self.block_size - 1) // self.block_size
 

@@ -88,17 +88,32 @@ class LocalExecutor:
 class Engine:
     def __init__(self, cfg: EngineConfig, executor=None, connector=None):
         self.cfg = cfg
+        self.blocks: BlockManager | None = None
+        self.connector = connector  # (refused before anything is loaded)
         self.executor = executor if executor is not None else LocalExecutor(cfg)
         self.blocks = BlockManager(self.executor.num_blocks, cfg.block_size)
         self.scheduler = Scheduler(self.blocks, cfg.max_batch, cfg.max_prefill_tokens, cfg.max_model_len)
-        if connector is not None and cfg.kv_quant is not None:
-            raise ValueError("the committed-KV store takes the unquantized K/V cache only")
-        self.connector = connector
         self._early: list[tuple[str, int | None, bool]] = []  # results a fork applied, for the next step()
         self.step_fn: Callable[[], list] = self._step
         self.last_plan: StepPlan | None = None
         self._ahead: _InFlight | None = None
         self.async_decode = bool(getattr(cfg, "async_decode", False)) and hasattr(self.executor, "launch_next")
+
+    @property
+    def connector(self):
+        """The KV connector called around each step, or None. A store commits the rows of the unquantized
+        cache and keeps them by their request, so it is refused on a 4-bit cache, and while forked requests
+        hold blocks together."""
+        return self._connector
+
+    @connector.setter
+    def connector(self, connector) -> None:
+        if connector is not None:
+            if getattr(self.cfg, "kv_quant", None) is not None:
+                raise ValueError("the committed-KV store takes the unquantized K/V cache only")
+            if self.blocks is not None and self.blocks.shared_blocks:
+                raise ValueError("forked requests hold cache blocks together: a store cannot be attached")
+        self._connector = connector
 
     # ---- requests --------------------------------------------------------------------------------
     def add_request(self, prompt: list[int], params: SamplingParams | None = None, req_id: str | None = None) -> str:

@@ -46,6 +46,35 @@ def test_config_refused():
         MultiprocExecutor(EngineConfig(TINY_LLAMA, device="cpu", kv_quant="int4"))
 
 
+def test_store_refused_however_attached(monkeypatch):
+    """A committed-KV store commits rows of the unquantized cache: no way of attaching one to a 4-bit cache, or to
+    requests that hold blocks together, is open, and a refused engine loads nothing."""
+    from everserve_b200.engine import engine as module
+    from everserve_b200.plugin import register
+
+    eng = _engine(kv_quant="int4")
+    with pytest.raises(ValueError):
+        register(eng, connector=object(), prepare=False)
+    with pytest.raises(ValueError):
+        eng.connector = object()
+    assert eng.connector is None
+    eng = _engine()
+    rid = eng.add_request(list(range(1, 20)), SamplingParams(max_tokens=8))
+    eng.step()
+    twin = eng.fork(rid)
+    with pytest.raises(ValueError):
+        register(eng, connector=object(), prepare=False)
+    while eng.has_work():
+        eng.step()
+    assert eng.request(twin).outputs == eng.request(rid).outputs
+    store = object()
+    register(eng, connector=store, prepare=False)
+    assert eng.connector is store
+    monkeypatch.setattr(module, "LocalExecutor", lambda cfg: pytest.fail("an executor was built"))
+    with pytest.raises(ValueError):
+        Engine(EngineConfig(TINY_LLAMA, device="cpu", dtype=torch.float32, num_blocks=8, kv_quant="int4"), connector=store)
+
+
 def test_shared_blocks():
     bm = BlockManager(4, 16)
     a = []
