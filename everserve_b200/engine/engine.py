@@ -134,7 +134,9 @@ class Engine:
         """Continue a running request a second time: a new request with its first `keep` tokens (default:
         all so far; its prompt's length draws every output anew) and its own `params` (default: the
         request's). Nothing is recomputed: the two hold the full cache blocks of the common tokens
-        together, and the block the new one writes into is copied. Call it between steps."""
+        together, and the block the new one writes into is copied. Where `params` asks for
+        log-probabilities, those of the outputs kept are the request's (which must have as many
+        alternatives). Call it between steps."""
         if not hasattr(self.executor, "copy_pages"):
             raise NotImplementedError("this executor does not copy cache blocks")
         if self.connector is not None:
@@ -146,6 +148,12 @@ class Engine:
             raise ValueError(f"keep must be 1 .. {parent.num_tokens}, got {keep}")
         n = min(keep, len(parent.prompt))
         req = Request(parent.prompt[:n], params or parent.params, outputs=parent.outputs[: keep - n])
+        k = req.params.logprobs
+        if k is not None and req.outputs:
+            if (parent.params.logprobs is None or parent.params.logprobs < k
+                    or len(parent.logprobs) < len(req.outputs)):
+                raise ValueError(f"request {req_id} has no log-probabilities of {k} alternatives for the outputs kept")
+            req.logprobs = [(lp, top[:k]) for lp, top in parent.logprobs[: len(req.outputs)]]
         if new_id is not None:
             req.req_id = new_id
         self.executor.copy_pages(self.scheduler.fork(parent, req, keep))

@@ -126,6 +126,37 @@ def test_fork_mid_way():
         eng.fork("nobody")
 
 
+def test_fork_keeps_log_probabilities():
+    """A fork's log-probabilities are its outputs', one by one, those it keeps among them; one that asks for what
+    the request does not have is refused."""
+    prompt = [3, 1, 4, 1, 5, 9, 2, 6]
+    eng = _engine()
+    rid = eng.add_request(prompt, SamplingParams(max_tokens=12, logprobs=2))
+    plain = eng.add_request(prompt, SamplingParams(max_tokens=12))
+    for _ in range(6):
+        eng.step()
+    twin, back = eng.fork(rid), eng.fork(rid, SamplingParams(max_tokens=12, logprobs=1), keep=11)
+    for args in ((plain, SamplingParams(max_tokens=12, logprobs=1)), (rid, SamplingParams(max_tokens=12, logprobs=3))):
+        with pytest.raises(ValueError):
+            eng.fork(*args)
+    while eng.has_work():
+        eng.step()
+    want = eng.request(rid)
+    assert len(want.logprobs) == 12
+    for other, k in ((twin, 2), (back, 1)):
+        req = eng.request(other)
+        assert req.outputs == want.outputs and len(req.logprobs) == 12
+        for (lp, top), (wlp, wtop) in zip(req.logprobs, want.logprobs):
+            assert abs(lp - wlp) < 1e-4 and [t for t, _ in top] == [t for t, _ in wtop[:k]]
+    silent = _engine()
+    rid = silent.add_request(prompt, SamplingParams(max_tokens=6, logprobs=2))
+    silent.step()
+    none = silent.fork(rid, SamplingParams(max_tokens=6))
+    while silent.has_work():
+        silent.step()
+    assert silent.request(none).logprobs == [] and silent.request(none).outputs == silent.request(rid).outputs
+
+
 def test_fork_limits_and_preemption():
     eng = _engine(max_batch=2, num_blocks=8)
     rid = eng.add_request(list(range(1, 40)), SamplingParams(max_tokens=40))
