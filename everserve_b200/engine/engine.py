@@ -136,7 +136,8 @@ class Engine:
         request's). Nothing is recomputed: the two hold the full cache blocks of the common tokens
         together, and the block the new one writes into is copied. Where `params` asks for
         log-probabilities, those of the outputs kept are the request's (which must have as many
-        alternatives). Call it between steps."""
+        alternatives); kept outputs that `params` would have ended at are refused. Call it between
+        steps."""
         if not hasattr(self.executor, "copy_pages"):
             raise NotImplementedError("this executor does not copy cache blocks")
         if self.connector is not None:

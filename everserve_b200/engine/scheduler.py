@@ -85,6 +85,8 @@ class Scheduler:
             raise ValueError(f"request {parent.req_id} is not running")
         if req.req_id in self.requests:
             raise ValueError(f"request {req.req_id} exists")
+        if req.outputs and req.done_generating():
+            raise ValueError(f"the outputs kept already end the request ({req.finish_reason()})")
         if len(self.running) >= self.max_batch:
             raise RuntimeError("the batch is full")
         if len(req.prompt) + req.params.max_tokens > self.max_model_len:

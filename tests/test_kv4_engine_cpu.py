@@ -157,6 +157,28 @@ def test_fork_keeps_log_probabilities():
     assert silent.request(none).logprobs == [] and silent.request(none).outputs == silent.request(rid).outputs
 
 
+def test_fork_of_outputs_that_end_it_is_refused():
+    """Kept outputs that reach the fork's max_tokens, or end with one of its stop ids, leave nothing to continue."""
+    eng = _engine()
+    rid = eng.add_request([3, 1, 4, 1, 5, 9, 2, 6], SamplingParams(max_tokens=12))
+    for _ in range(5):
+        eng.step()
+    eng.flush()
+    out = list(eng.request(rid).outputs)
+    last = dict(max_tokens=12, stop_ids=(out[-1],))
+    for params in (SamplingParams(max_tokens=len(out)), SamplingParams(max_tokens=2), SamplingParams(**last),
+                   SamplingParams(max_tokens=12, eos_id=out[-1], ignore_eos=False)):
+        with pytest.raises(ValueError):
+            eng.fork(rid, params)
+    assert len(eng.scheduler.running) == 1 and eng.blocks.shared_blocks == 0
+    one = eng.fork(rid, SamplingParams(max_tokens=len(out) + 1))
+    two = eng.fork(rid, SamplingParams(max_tokens=2), keep=9)
+    while eng.has_work():
+        eng.step()
+    want = eng.request(rid).outputs
+    assert eng.request(one).outputs == want[: len(out) + 1] and eng.request(two).outputs == want[:2]
+
+
 def test_fork_limits_and_preemption():
     eng = _engine(max_batch=2, num_blocks=8)
     rid = eng.add_request(list(range(1, 40)), SamplingParams(max_tokens=40))
