@@ -324,20 +324,23 @@ class Engine:
         return [self.scheduler.requests[i].outputs for i in ids]
 
     def samples(self, prompt: list[int], n: int, max_tokens: int = 16, **sampling) -> list[list[int]]:
-        """n completions of one prompt, which is prefilled once: the others are forked from it. `sampling`
-        as in `generate`; with a seed, completion i takes seed + i."""
+        """n completions of one prompt. The prompt is prefilled once and the others are forked from it, as many
+        as the batch and the cache have room for while the first one runs (with max_tokens=1 it ends with the
+        prefill); the rest, and all of them on an engine that cannot fork (with a store, or an executor that
+        does not copy blocks), prefill the prompt themselves. `sampling` as in `generate`; with a seed,
+        completion i takes seed + i."""
         if n < 1:
             raise ValueError("n must be at least 1")
         seed = sampling.pop("seed", None)
         each = [SamplingParams(max_tokens=max_tokens, seed=None if seed is None else seed + i, **sampling) for i in range(n)]
         first = self.add_request(prompt, each[0])
         req = self.scheduler.requests[first]
-        while not req.outputs:
+        forks = n > 1 and self.connector is None and hasattr(self.executor, "copy_pages")
+        while forks and not req.outputs:
             self.step()
         ids = [first]
         for p in each[1:]:
-            # a batch without room, or a request that ended meanwhile: the prompt by itself
-            if req.status is Status.RUNNING and len(self.scheduler.running) < self.cfg.max_batch and self.blocks.free_blocks:
+            if forks and req.status is Status.RUNNING and len(self.scheduler.running) < self.cfg.max_batch and self.blocks.free_blocks:
                 ids.append(self.fork(first, p, keep=len(prompt)))
             else:
                 ids.append(self.add_request(prompt, p))

@@ -104,6 +104,47 @@ def test_samples_are_their_seeds_own_runs(kv, plen):
     assert got == alone and got[0] != got[1]
 
 
+class _Store:
+    """A connector that watches."""
+
+    def begin_step(self, plan, scheduler):
+        pass
+
+    end_step = begin_step
+
+    def finished(self, req_id):
+        pass
+
+
+class _Apart:
+    """An executor that runs plans and copies no blocks."""
+
+    def __init__(self, inner):
+        self.inner, self.num_blocks = inner, inner.num_blocks
+
+    def execute(self, plan):
+        return self.inner.execute(plan)
+
+    def fetch(self, ids):
+        return self.inner.fetch(ids)
+
+
+@pytest.mark.parametrize("how", ["store", "executor", "one token", "small batch"])
+def test_samples_where_not_all_are_forks(how):
+    """Completions that cannot be forked prefill the prompt themselves; no request is left behind."""
+    prompt = [(5 * i + 2) % 500 for i in range(19)]
+    kw = dict(max_tokens=1 if how == "one token" else 6, temperature=0.9, top_k=20, seed=3)
+    eng = _engine(max_batch=2 if how == "small batch" else 4)
+    if how == "store":
+        eng.connector = _Store()
+    if how == "executor":
+        eng.executor, eng.async_decode = _Apart(eng.executor), False
+    got = eng.samples(prompt, 5, **kw)
+    assert not eng.has_work() and eng.blocks.free_blocks == 64
+    seed = kw.pop("seed")
+    assert got == [_engine().generate([prompt], seed=seed + i, **kw)[0] for i in range(5)]
+
+
 def test_fork_mid_way():
     """A fork of a request under way continues as the request does; one from an earlier token replays it;
     results the fork had to apply come with the next step."""
