@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
   uint32_t taken = 0;
   auto next_item = [&]() {
     const int s = taken & 1;
-    ok = __all_sync(0xffffffffu, wait_for(&item_full[s], (taken >> 1) & 1));
+    ok = __all_sync(0xffffffffu, wait_for(&item_full[s], (taken >> 1) & 1)) && ok;
     if (!ok) return false;
     it = s_item[s];
     __syncwarp();
