@@ -299,17 +299,20 @@ struct Kv4PrefillArgs {
   const int* ctx_lens;
   const int64_t* last_rows;
   void* out;       // [T, hq, d]
-  float* part_o;   // [T, hq, max_splits, d] (unused with one split)
-  float* part_ml;  // [T, hq, max_splits, 2]
-  int* part_ns;    // [T]
+  int64_t parts;   // rows times splits that the workspace holds; a sequence beyond them is not cut
+  float* part_o;   // [parts * hq, d], 16-byte aligned (unused where parts is 0, as the next two)
+  float* part_ml;  // [parts * hq, 2]
+  void* part_at;   // [T] pairs of 32 bits
   unsigned* next;  // a word the launch zeroes
   int* status;
   int64_t T, S;
-  int hq, max_splits, num_sms;
+  int hq, num_sms;
   float scale;
 };
-// splits a row of such a step may be cut into, with no context above max_len
-int64_t kv4_prefill_splits(int64_t T, int64_t S, int64_t hq, int64_t hkv, int64_t max_len);
+// Rows times splits of such a step: of each sequence's new rows and context length (host arrays of S), or, where they
+// are null, the most with no context above max_len (a lone sequence owning all the rows).
+int64_t kv4_prefill_parts(int64_t T, int64_t S, int64_t hq, int64_t hkv, int64_t max_len, const int64_t* rows,
+                          const int64_t* ctx);
 cudaError_t launch_kv4_prefill(const Kv4PrefillArgs& a, cudaStream_t s);
 // pages (blocks) of every layer's cache copied, pairs [n, 2] = (from, to), < 0: padding
 struct CopyPagesArgs {

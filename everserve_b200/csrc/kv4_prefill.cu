@@ -36,6 +36,7 @@
 // 654 us; instructions bound the softmax, not the exponential unit.) 16 prompts of 8191 rows in all take 119 us:
 // an item of three key tiles pays as much again for its query, its first conversion and its output. Two more
 // warps that copied the next item's query ahead made that 130 us.
+#include <algorithm>
 #include <atomic>
 #include <climits>
 
@@ -94,26 +95,41 @@ struct PreParams {
   const int* ctx_lens;
   const int64_t* last_rows;
   __nv_bfloat16* out;  // [T, hq, D]
-  float* part_o;       // [T, hq, max_splits, D]
-  float* part_ml;      // [T, hq, max_splits, 2]
-  int* part_ns;        // [T]
+  float* part_o;       // [parts * hq, D]: a row's parts head by head
+  float* part_ml;      // [parts * hq, 2]
+  uint2* part_at;      // [T]: (its parts | its sequence's << 16, its first part's row); null: nothing is cut
   int* status;
   unsigned* next;      // items handed out beyond each CTA's first, zero before the launch
-  int T, S, hq, hkv, G, tt, max_splits;  // tt: tokens of a 128-row tile
+  int T, S, hq, hkv, G, tt;  // tt: tokens of a 128-row tile
+  int parts;                 // rows times splits that the workspace holds
   float scale_log2;
 };
 
-// Key tiles of one item for a sequence of `tiles` row tiles: all of them where its items fill the SMs
-// without a cut.
-__host__ __device__ __forceinline__ int chunk_of(int tiles, int hkv) {
+// How a sequence of `tiles` row tiles and `keys` key tiles is cut along its keys: the key tiles of an item, and the
+// items that a row tile has at most. Not at all where its row tiles fill the SMs; else into kCutItems items at most, which
+// bounds its parts in the workspace whatever its length (256 rows of a head an item: 34 to 51 MB at head dim 128).
+// (64 rows on 131K keys, 32 / 8 heads of 128: 203 us, without the bound 245; 900 rows on 60K: 1,265 and 1,237; 509 rows on 0-40K keys, 14 / 2 of 64: 106 and 107.)
+struct Cut {
+  int chunk, splits;
+};
+constexpr int kCutItems = 256;
+__host__ __device__ __forceinline__ int least_chunk(int items) { return items > 16 ? 16 : 8; }
+__host__ __device__ __forceinline__ int most_splits(int items) { return (kCutItems + items - 1) / items; }
+__host__ __device__ __forceinline__ Cut cut_of(int tiles, int hkv, int keys) {
   const int items = tiles * hkv;
-  return items >= 128 ? 1 << 24 : items > 16 ? 16 : 8;
+  Cut c{1 << 24, 1};
+  if (items == 0 || items >= 128 || keys <= 0) return c;
+  const int least = least_chunk(items), most = most_splits(items), fair = (keys + most - 1) / most;
+  c.chunk = least > fair ? least : fair;
+  c.splits = (keys + c.chunk - 1) / c.chunk;
+  return c;
 }
 
 struct Item {
   int seq, rows, row0, ctx;  // the sequence, its rows, its first row, its context length
   int tile, head, split, chunk;
   int j0, j1, ns;  // its key tiles, and how many items its row tile has
+  int per, part0;  // the sequence's splits, and its first row in the workspace
 };
 
 // Work item `idx`, in an order that puts long ones first: of 32 sequences at a time those with the most keys,
@@ -121,6 +137,7 @@ struct Item {
 ES_DEVICE bool find_item(const PreParams& p, int bs, int idx, Item& it) {
   const int lane = threadIdx.x & 31;
   int before = 0;
+  int64_t parts = 0;  // of the sequences before these 32
 #pragma unroll 1
   for (int s0 = 0; s0 < p.S; s0 += 32) {
     const int s = s0 + lane;
@@ -131,10 +148,26 @@ ES_DEVICE bool find_item(const PreParams& p, int bs, int idx, Item& it) {
       rows = max(0, (int)min(T, p.last_rows[s] + 1) - r0);
       ctx = min(p.ctx_lens[s], p.bt_cols * bs);
       tiles = (rows + 2 * p.tt - 1) / (2 * p.tt);
-      chunk = chunk_of(tiles, p.hkv);
-      ns = max(1, min(p.max_splits, ((ctx + kKeys - 1) / kKeys + chunk - 1) / chunk));
-      items = tiles * ns * p.hkv;
+      const Cut c = cut_of(tiles, p.hkv, (ctx + kKeys - 1) / kKeys);
+      chunk = c.chunk, ns = c.splits;
     }
+    // its place in the workspace; one that the workspace has no room for is not cut
+    int part0 = 0;
+    if (p.parts > 0) {
+      const int need = ns > 1 ? rows * ns : 0;
+      int sum = need;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += v;
+      }
+      part0 = (int)min(parts + sum - need, (int64_t)p.parts);
+      if (parts + sum > p.parts) chunk = 1 << 24, ns = 1;
+      parts += __shfl_sync(0xffffffffu, sum, 31);
+    } else {
+      chunk = 1 << 24, ns = 1;
+    }
+    items = tiles * ns * p.hkv;
     // this lane's place in the order: the sequence (lane) `src`
     int src = lane;
     if (p.S > 1) {
@@ -166,6 +199,8 @@ ES_DEVICE bool find_item(const PreParams& p, int bs, int idx, Item& it) {
       it.ctx = __shfl_sync(0xffffffffu, ctx, src);
       it.chunk = __shfl_sync(0xffffffffu, chunk, src);
       const int t = __shfl_sync(0xffffffffu, tiles, src), per = __shfl_sync(0xffffffffu, ns, src);
+      it.per = per;
+      it.part0 = __shfl_sync(0xffffffffu, part0, src);
       const uint32_t at = idx - first, group = at / (uint32_t)p.hkv, splits = (uint32_t)per;
       it.tile = t - 1 - (int)(group / splits);
       it.split = (int)(group % splits);
@@ -182,7 +217,7 @@ ES_DEVICE void span(const PreParams& p, Item& it) {
   const int last = min(it.rows, (it.tile + 1) * 2 * p.tt) - 1;  // the tile's last token
   const int pos = min(it.ctx - it.rows + last, it.ctx - 1);
   const int J = pos < 0 ? 0 : pos / kKeys + 1;
-  it.ns = max(1, min(p.max_splits, (J - 1) / it.chunk + 1));
+  it.ns = max(1, (J - 1) / it.chunk + 1);
   it.j0 = it.split * it.chunk;
   it.j1 = it.split == it.ns - 1 ? J : min(J, it.j0 + it.chunk);
   if (it.split >= it.ns) it.j1 = it.j0;
@@ -466,7 +501,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
       for (int64_t x = max((int64_t)0, p.last_rows[p.S - 1] + 1) + blockIdx.x; x < p.T; x += gridDim.x) {
         uint4* row = reinterpret_cast<uint4*>(p.out) + x * vecs;
         for (int i = threadIdx.x & 63; i < vecs; i += 64) row[i] = make_uint4(0, 0, 0, 0);
-        if ((threadIdx.x & 63) == 0 && p.part_ns != nullptr) p.part_ns[x] = 1;
+        if ((threadIdx.x & 63) == 0 && p.part_at != nullptr) p.part_at[x] = make_uint2(1, 0);
       }
     }
     const bool failed = !ok;
@@ -576,7 +611,10 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
       const int64_t q_at = real ? (int64_t)(it.row0 + at) * p.q_stride + (it.head * p.G + head) * D : -1;
       const int64_t out_row = real ? (int64_t)(it.row0 + at) * p.hq + it.head * p.G + head : -1;
       const int pos = it.ctx - it.rows + at;
-      if (real && it.split == 0 && it.head == 0 && head == 0 && p.part_ns != nullptr) p.part_ns[it.row0 + at] = ns;
+      // its place in the workspace: the row's parts, head by head
+      const int part = ns > 1 ? (it.part0 + at * it.per) * p.hq + (it.head * p.G + head) * it.per + it.split : 0;
+      if (real && it.split == 0 && it.head == 0 && head == 0 && p.part_at != nullptr)
+        p.part_at[it.row0 + at] = ns > 1 ? make_uint2(ns | it.per << 16, it.part0 + at * it.per) : make_uint2(1, 0);
       if (j0 >= j1) {
         if (it.split == 0 && real)  // no key at all
           for (int i = 0; i < U; i++) reinterpret_cast<uint4*>(p.out + out_row * D)[i] = make_uint4(0, 0, 0, 0);
@@ -722,7 +760,6 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
       const float scale_o = ns > 1 ? unit_o : none ? 0.f : unit_o / l;
       // a row that sees a V of NaN, by halves of the channels
       const float scale0 = hole0 ? NAN : scale_o, scale1 = hole1 ? NAN : scale_o;
-      const int64_t part = out_row * p.max_splits + it.split;
       if (ns == 1) {
 #pragma unroll 1
         for (int q = 0; q < D / 32; q++) {
@@ -767,14 +804,14 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(PreParams p) {
 #pragma unroll 4
           for (int x = 0; x < 8; x++) {
             const int from = x * 4 + lane / 8;
-            const int64_t to = __shfl_sync(0xffffffffu, real ? part : -1, from);
+            const int to = __shfl_sync(0xffffffffu, real ? part : -1, from);
             const float4 y = *cell(w0 + from, lane & 7);
-            if (to >= 0) reinterpret_cast<float4*>(p.part_o + to * D + q * 32)[lane & 7] = y;
+            if (to >= 0) reinterpret_cast<float4*>(p.part_o + (int64_t)to * D + q * 32)[lane & 7] = y;
           }
           __syncwarp();
         }
       }
-      if (real && ns > 1) p.part_ml[2 * part] = m, p.part_ml[2 * part + 1] = l;
+      if (real && ns > 1) reinterpret_cast<float2*>(p.part_ml)[part] = make_float2(m, l);
       ptx::tc_fence_before();
     }
     if (!ok) s_fail = 1;
@@ -795,16 +832,18 @@ __global__ void __launch_bounds__(128) prefill_merge_kernel(PreParams p) {
   const int64_t rh = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (rh >= (int64_t)p.T * p.hq) return;
-  const int ns = min(p.part_ns[rh / p.hq], p.max_splits);
+  const uint2 of = p.part_at[rh / p.hq];
+  const int ns = of.x & 0xFFFF, per = of.x >> 16;
   if (ns <= 1) return;
-  const float* ml = p.part_ml + rh * p.max_splits * 2;
+  const int64_t part = (int64_t)of.y * p.hq + rh % p.hq * per;
+  const float* ml = p.part_ml + part * 2;
   float mx = -INFINITY;
   for (int i = lane; i < ns; i += 32) mx = fmaxf(mx, ml[2 * i]);
   mx = warp_max(mx);
   float acc[E], l = 0.f;
 #pragma unroll
   for (int e = 0; e < E; e++) acc[e] = 0.f;
-  const float* po = p.part_o + rh * p.max_splits * D + E * lane;  // a lane E neighbouring channels
+  const float* po = p.part_o + part * D + E * lane;  // a lane E neighbouring channels
 #pragma unroll 4
   for (int i = 0; i < ns; i++) {
     const float2 t = reinterpret_cast<const float2*>(ml)[i];
@@ -836,27 +875,49 @@ cudaError_t launch_prefill(const PreParams& p, int grid, cudaStream_t stream) {
   });
   if (e != cudaSuccess) return e;
   e = launch_ex(prefill_kernel<D, NG, BS>, dim3(grid), dim3(kPreThreads), PreCfg<D>::kSmem, stream, 0, p);
-  if (e != cudaSuccess || p.max_splits == 1) return e;
+  if (e != cudaSuccess || p.parts == 0) return e;
   return launch_ex(prefill_merge_kernel<D>, dim3((unsigned)(((int64_t)p.T * p.hq + 3) / 4)), dim3(128), 0, stream, 0, p);
 }
 
 }  // namespace kv4
 
-int64_t kv4_prefill_splits(int64_t T, int64_t S, int64_t hq, int64_t hkv, int64_t max_len) {
-  if (T <= 0 || S <= 0 || hkv <= 0 || hq < hkv || hq / hkv > kv4::kRows) return 1;
-  const int64_t J = (max_len + kv4::kKeys - 1) / kv4::kKeys;
+int64_t kv4_prefill_parts(int64_t T, int64_t S, int64_t hq, int64_t hkv, int64_t max_len, const int64_t* rows,
+                          const int64_t* ctx) {
+  if (T <= 0 || S <= 0 || hkv <= 0 || hq < hkv || hq / hkv > kv4::kRows) return 0;
   const int64_t tt2 = 2 * (kv4::kRows / (hq / hkv));
-  // one sequence: its rows are the step's; several: one of them may have as few as one
-  const int chunk = kv4::chunk_of(S == 1 ? (int)((T + tt2 - 1) / tt2) : 1, (int)hkv);
-  return J <= chunk ? 1 : (J + chunk - 1) / chunk;
+  const auto tiles_of = [&](int64_t r) { return (int)std::min<int64_t>((r + tt2 - 1) / tt2, 128); };
+  const auto keys_of = [](int64_t n) { return (int)((std::min<int64_t>(n, INT32_MAX - kv4::kKeys) + kv4::kKeys - 1) / kv4::kKeys); };
+  // splits of a sequence of t row tiles and any context up to that of k key tiles
+  const auto splits = [&](int t, int k) {
+    const int64_t items = t * hkv;
+    return items >= 128 ? 1 : (int64_t)std::min((k + kv4::least_chunk(items) - 1) / kv4::least_chunk(items), kv4::most_splits(items));
+  };
+  if (rows != nullptr) {
+    int64_t sum = 0;
+    for (int64_t s = 0; s < S; s++) {
+      if (rows[s] <= 0 || ctx[s] <= 0) continue;
+      const int64_t n = tiles_of(rows[s]) * hkv >= 128 ? 1 : kv4::cut_of(tiles_of(rows[s]), (int)hkv, keys_of(ctx[s])).splits;
+      if (n > 1) sum += rows[s] * n;
+    }
+    return sum;
+  }
+  const int k = keys_of(max_len);
+  if (S == 1) return splits(tiles_of(T), k) > 1 ? T * splits(tiles_of(T), k) : 0;  // its rows are the step's
+  // each sequence may be of the length that takes the most, and each row of the one that is cut the most
+  int64_t seq = 0, row = 0;
+  for (int t = 1; t <= tiles_of(T) && t * hkv < 128; t++) {
+    const int64_t n = splits(t, k);
+    if (n > 1) seq = std::max(seq, t * tt2 * n), row = std::max(row, n);
+  }
+  return std::min(S * seq, T * row);
 }
 
 cudaError_t launch_kv4_prefill(const Kv4PrefillArgs& a, cudaStream_t stream) {
   if (a.T == 0) return cudaSuccess;
   if (a.S == 0) return cudaMemsetAsync(a.out, 0, (size_t)a.T * a.hq * a.c.d * sizeof(__nv_bfloat16), stream);
-  if (a.c.hkv <= 0 || a.hq % a.c.hkv != 0 || a.hq / a.c.hkv > kv4::kRows || a.max_splits < 1 || !(a.scale > 0.f))
+  if (a.c.hkv <= 0 || a.hq % a.c.hkv != 0 || a.hq / a.c.hkv > kv4::kRows || a.parts < 0 || !(a.scale > 0.f))
     return cudaErrorInvalidValue;
-  if (a.c.s_block >> 4 > UINT32_MAX) return cudaErrorInvalidValue;
+  if (a.c.s_block >> 4 > UINT32_MAX || a.parts * a.hq > INT32_MAX) return cudaErrorInvalidValue;
   if (a.T > INT32_MAX / 2 || a.bt_cols * a.c.block_size > INT32_MAX - kv4::kKeys || a.T * a.hq > ((int64_t)1 << 32))
     return cudaErrorInvalidValue;
   kv4::PreParams p{};
@@ -873,7 +934,7 @@ cudaError_t launch_kv4_prefill(const Kv4PrefillArgs& a, cudaStream_t stream) {
   p.out = static_cast<__nv_bfloat16*>(a.out);
   p.part_o = a.part_o;
   p.part_ml = a.part_ml;
-  p.part_ns = a.max_splits > 1 ? a.part_ns : nullptr;
+  p.part_at = a.parts > 0 ? static_cast<uint2*>(a.part_at) : nullptr;
   p.next = a.next;
   p.status = a.status;
   p.T = (int)a.T;
@@ -882,11 +943,11 @@ cudaError_t launch_kv4_prefill(const Kv4PrefillArgs& a, cudaStream_t stream) {
   p.hkv = a.c.hkv;
   p.G = a.hq / a.c.hkv;
   p.tt = kv4::kRows / p.G;
-  p.max_splits = a.max_splits;
+  p.parts = (int)a.parts;
   p.scale_log2 = a.scale * 1.4426950408889634f;
-  // items: at most a row tile per 2 tt rows and sequence, each times heads and splits
-  const int64_t most = (a.T / (2 * p.tt) + a.S) * p.hkv * a.max_splits;
-  const int grid = (int)(most < a.num_sms ? most : a.num_sms);
+  // items: at most a row tile per 2 tt rows and sequence, each times heads, and more where some are cut
+  const int64_t most = (a.T / (2 * p.tt) + a.S) * p.hkv;
+  const int grid = (int)(a.parts == 0 && most < a.num_sms ? most : a.num_sms);
   const cudaError_t e = cudaMemsetAsync(a.next, 0, sizeof(unsigned), stream);
   if (e != cudaSuccess) return e;
   return kv4::pick(a.c.d, a.c.groups, a.c.block_size, [&](auto d, auto ng, auto bs) {

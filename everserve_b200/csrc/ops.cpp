@@ -836,13 +836,16 @@ torch::Tensor paged_decode_kv4(torch::Tensor q, torch::Tensor cache, torch::Tens
 
 torch::Tensor paged_prefill_kv4(torch::Tensor q, torch::Tensor cache, torch::Tensor block_tables,
                                 torch::Tensor ctx_lens, torch::Tensor last_rows, torch::Tensor status,
-                                int64_t block_size, int64_t max_context, double scale, int64_t num_sms) {
+                                int64_t block_size, int64_t max_context, double scale, int64_t num_sms,
+                                c10::optional<std::vector<std::pair<int64_t, int64_t>>> lengths) {
   check_bf16(q, "q");
   TORCH_CHECK(q.dim() == 3, "q must be [T, hq, head_dim]");
   on_device_of(last_rows, at::kLong, q, "last_rows: int64 on the device of q");
   TORCH_CHECK(last_rows.dim() == 1 && last_rows.is_contiguous(), "last_rows: one contiguous value per sequence");
   TORCH_CHECK(scale > 0, "scale must be positive");
   TORCH_CHECK(max_context >= 1 && num_sms >= 1, "max_context and num_sms must be positive");
+  TORCH_CHECK(!lengths.has_value() || (int64_t)lengths->size() == last_rows.numel(),
+              "lengths: (new rows, context length) of each sequence");
   const int64_t T = q.size(0), S = last_rows.numel(), hq = q.size(1), d = q.size(2);
   es::Kv4PrefillArgs a{};
   a.c = kv4_attention_args(q, cache, block_tables, ctx_lens, status, S, block_size);
@@ -865,14 +868,17 @@ torch::Tensor paged_prefill_kv4(torch::Tensor q, torch::Tensor cache, torch::Ten
   torch::Tensor next = torch::empty({1}, q.options().dtype(at::kInt));
   a.out = out.data_ptr();
   a.next = reinterpret_cast<unsigned*>(next.data_ptr<int>());
-  const int64_t splits =
-      es::kv4_prefill_splits(T, S, hq, a.c.hkv, std::min<int64_t>(max_context, block_tables.size(1) * block_size));
-  a.max_splits = (int)splits;
-  if (splits > 1) {
-    part = torch::empty({T * hq * splits * (d + 2) + T}, q.options().dtype(at::kFloat));
+  std::vector<int64_t> rows, ctx;
+  if (lengths.has_value()) {
+    for (const auto& l : *lengths) rows.push_back(l.first), ctx.push_back(l.second);
+  }
+  a.parts = es::kv4_prefill_parts(T, S, hq, a.c.hkv, std::min<int64_t>(max_context, block_tables.size(1) * block_size),
+                                  lengths.has_value() ? rows.data() : nullptr, ctx.data());
+  if (a.parts > 0) {
+    part = torch::empty({a.parts * hq * (d + 2) + 2 * T}, q.options().dtype(at::kFloat));
     a.part_o = part.data_ptr<float>();
-    a.part_ml = a.part_o + T * hq * splits * d;
-    a.part_ns = reinterpret_cast<int*>(a.part_ml + T * hq * splits * 2);
+    a.part_ml = a.part_o + a.parts * hq * d;
+    a.part_at = a.part_ml + a.parts * hq * 2;
   }
   ES_CHECK_CUDA(es::launch_kv4_prefill(a, cur()));
   return out;

@@ -187,7 +187,8 @@ class ModelRunner:
         tiles = prefill_tiles(seq, pos, device=dev) if plan_tiles else None
         return StepInput(ids=t(ids), positions=t(pos), slots=t(slots), block_tables=bt.to(dev),
                          ctx_lens=t(ctx, torch.int32), q_seq=t(seq), logits_idx=t(last), is_decode=False,
-                         max_model_len=self.max_model_len, sampling=sb, prefill_tiles=tiles, max_context=max(ctx))
+                         max_model_len=self.max_model_len, sampling=sb, prefill_tiles=tiles,
+                         max_context=max(ctx), lengths=[(len(r.token_ids), n) for r, n in zip(plan.reqs, ctx)])
 
     def copy_pages(self, pairs: list[tuple[int, int]]) -> None:
         """Copy blocks (from, to) in every layer's cache, behind the work enqueued so far."""

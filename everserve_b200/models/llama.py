@@ -44,6 +44,7 @@ class StepInput:
     logprobs_k: int | None = None  # the step also reports log-probabilities (k alternatives)
     prefill_tiles: torch.Tensor | None = None  # prefill kernel work list (ops.prefill_tiles), device
     max_context: int | None = None  # the largest context length, where the host knows it
+    lengths: list | None = None  # each sequence's (new rows, context length), where the host knows them
 
 
 def _seed_of(seed: int, *parts) -> int:
@@ -315,7 +316,7 @@ class DecoderLM:
             return ops.decode_attention_kv4(q, cache, inp.block_tables, inp.ctx_lens, self.scale, bs,
                                             inp.max_model_len or None)
         return ops.prefill_attention_kv4(q, cache, inp.block_tables, inp.ctx_lens, inp.logits_idx, self.scale, bs,
-                                         inp.max_context)
+                                         inp.max_context, inp.lengths)
 
     # ---- forward -------------------------------------------------------------------------------
     def embed(self, ids: torch.Tensor) -> torch.Tensor:

@@ -74,7 +74,8 @@ class RefOps:
         rows = torch.arange(q.shape[0], device=q.device)
         return ref.kv4_attention(q, cache, block_tables, ctx_lens[: q.shape[0]], rows, scale, block_size)
 
-    def prefill_attention_kv4(self, q, cache, block_tables, ctx_lens, last_rows, scale, block_size, max_context=None):
+    def prefill_attention_kv4(self, q, cache, block_tables, ctx_lens, last_rows, scale, block_size, max_context=None,
+                              lengths=None):
         return ref.kv4_attention(q, cache, block_tables, ctx_lens, last_rows, scale, block_size)
 
     def copy_pages(self, caches, pairs):
@@ -286,16 +287,20 @@ class KernelOps:
             max_model_len = block_tables.shape[1] * block_size
         return self.C.paged_decode_kv4(q, cache, block_tables, ctx_lens, self.status, block_size, max_model_len, scale)
 
-    def prefill_attention_kv4(self, q, cache, block_tables, ctx_lens, last_rows, scale, block_size, max_context=None):
+    def prefill_attention_kv4(self, q, cache, block_tables, ctx_lens, last_rows, scale, block_size, max_context=None,
+                              lengths=None):
         """Causal attention of a step's new rows over their sequences' history in 4 bits (the rows' own
         keys and values written before): sequence s owns the rows up to last_rows[s] (int64, on the
         device), the last of them at position ctx_lens[s] - 1. q [T, hq, d] -> [T, hq, d]; a row without a
-        visible key, or past the last sequence's, gives zeros. `max_context` bounds the step's context lengths (default: what
-        block_tables can hold); it sizes the call's own workspace, nothing else."""
+        visible key, or past the last sequence's, gives zeros. A sequence of few rows and
+        a long history is cut along its keys, and its parts take workspace of the call's own. `lengths`, each
+        sequence's (new rows, context length) on the host, sizes it by what this step needs; without them it
+        is sized for the worst step with no context above `max_context` (default: what block_tables can hold). A
+        sequence that they leave no room for is not cut: slower, and as right."""
         if max_context is None:
             max_context = block_tables.shape[1] * block_size
         return self.C.paged_prefill_kv4(q, cache, block_tables, ctx_lens, last_rows, self.status, block_size,
-                                        max_context, scale, self.num_sms)
+                                        max_context, scale, self.num_sms, lengths)
 
     def copy_pages(self, caches, pairs):
         """Copy pages (the first dimension's entries) in every layer's cache, bf16 or 4-bit: pairs int64

@@ -240,3 +240,11 @@ def test_fork_limits_and_preemption():
     tight.step()
     with pytest.raises(MemoryError):
         tight.fork(rid)
+
+
+def test_prefill_step_carries_its_lengths():
+    eng = _engine(kv_quant="int4")
+    for n in (19, 3):
+        eng.add_request(list(range(1, n + 1)), SamplingParams(max_tokens=4))
+    inp = eng.executor.worker.runner.prefill_input(eng.scheduler.schedule())
+    assert inp.lengths == [(19, 19), (3, 3)] and inp.max_context == 19

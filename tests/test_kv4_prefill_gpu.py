@@ -117,3 +117,48 @@ def test_visible_scores_of_minus_infinity(kops):
     out = kops.prefill_attention_kv4(q, cache, tables, ctx, last, 0.1, bs)
     assert bool(out[:, 0].isnan().all()) and bool(torch.isfinite(out[:, 1]).all())
     assert kops.check_status() == 0
+
+
+def test_workspace_is_what_the_step_needs(kops):
+    """A prompt that is not cut beside one row over a long history: 65 MB of output, and no workspace to speak of
+    when the lengths are given; without them no more than two sequences can take. Results do not move."""
+    hq, hkv, d, group, bs = 32, 8, 128, 64, 16
+    rows, lens = [8000, 1], [8000, 8001]
+    q, cache, tables, ctx, last = batch(lens, rows, hq, hkv, d, group, bs, 44)
+    outs = []
+    for lengths, most in ((None, 200 << 20), (list(zip(rows, lens)), 2 << 20)):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        kw = {} if lengths is None else dict(lengths=lengths)
+        outs.append(kops.prefill_attention_kv4(q, cache, tables, ctx, last, 0.1, bs, **kw))
+        assert torch.cuda.max_memory_allocated() - before <= q.numel() * 2 + most
+    assert torch.equal(*outs)
+    one = kops.prefill_attention_kv4(q[8000:], cache, tables[1:], ctx[1:], last[1:] - 8000, 0.1, bs)
+    assert torch.equal(one, outs[0][8000:])
+    # 16 sequences of 128 rows on 16K keys: each at most 51 MB of parts
+    q, cache, tables, ctx, last = batch([16400 + i for i in range(16)], [128] * 16, hq, hkv, d, group, bs, 45)
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    full = kops.prefill_attention_kv4(q, cache, tables, ctx, last, 0.1, bs)
+    assert torch.cuda.max_memory_allocated() - before <= 16 * (51 << 20)
+    del full
+    assert kops.check_status() == 0
+
+
+def test_lengths_that_fall_short_are_safe(kops):
+    """Lengths below the step's leave sequences uncut, with the same values within the roundings."""
+    hq, hkv, d, group, bs = 8, 2, 128, 64, 16
+    rows, lens = [5, 40, 1, 30], [3000, 2500, 4000, 200]
+    q, cache, tables, ctx, last = batch(lens, rows, hq, hkv, d, group, bs, 46)
+    want, mag = oracle(q, cache, tables, ctx, last, 0.1, bs)
+    tol = bound(q, cache, tables, ctx, last, 0.1, bs, want, mag)
+    full = kops.prefill_attention_kv4(q, cache, tables, ctx, last, 0.1, bs)
+    held_to(full, want, tol)
+    assert torch.equal(full, kops.prefill_attention_kv4(q, cache, tables, ctx, last, 0.1, bs, lengths=list(zip(rows, lens))))
+    for lengths in ([(0, 0)] * 4, [(5, 3000), (0, 0), (0, 0), (0, 0)], [(1, 2048)] * 4):
+        held_to(kops.prefill_attention_kv4(q, cache, tables, ctx, last, 0.1, bs, lengths=lengths), want, tol)
+    for bad in ([(5, 3000)], []):
+        with pytest.raises(RuntimeError):
+            kops.prefill_attention_kv4(q, cache, tables, ctx, last, 0.1, bs, lengths=bad)
+    assert kops.check_status() == 0
