@@ -162,3 +162,106 @@ def test_lengths_that_fall_short_are_safe(kops):
         with pytest.raises(RuntimeError):
             kops.prefill_attention_kv4(q, cache, tables, ctx, last, 0.1, bs, lengths=bad)
     assert kops.check_status() == 0
+
+
+# Over many values of long histories, where an output is a small part of A: bf16's rounding has 0.0017 of the norm. P's
+# and V's roundings are noise of u / sqrt 3 times 0.75 (a value's place in its binade) of what they round, 2.1e-4 each. A
+# key's moves its score by 2.1e-4 sqrt(d) scale sqrt(5) = 4.7e-4 (these keys have a second moment of 5), and the output by as
+# much of itself. Half as much again is allowed.
+AVERAGE = 1.5 * (0.0017**2 + 2 * 0.00021**2 + 0.00047**2) ** 0.5
+
+
+@pytest.mark.parametrize("hq,hkv,d,group,bs", [(32, 8, 128, 64, 16), (32, 8, 128, 128, 32), (14, 2, 64, 64, 16)])
+def test_averages_of_long_histories(kops, hq, hkv, d, group, bs):
+    """Histories cut along their keys (40 rows on 40K) and whole (1100 rows on 4K)."""
+    rows, lens = [40, 1100], [40040, 5100]
+    q, cache, tables, ctx, last = batch(lens, rows, hq, hkv, d, group, bs, 51)
+    out = kops.prefill_attention_kv4(q, cache, tables, ctx, last, d**-0.5, bs)
+    want, _ = oracle(q, cache, tables, ctx, last, d**-0.5, bs)
+    for part in (slice(0, 40), slice(40, None)):
+        assert float((out[part].double() - want[part]).norm() / want[part].norm()) < AVERAGE
+    assert kops.check_status() == 0
+
+
+@pytest.mark.parametrize("hq,hkv,d,group,bs", LAYOUTS)
+def test_sizes_far_apart(kops, hq, hkv, d, group, bs):
+    """Pages whose values are 2^15 and 2^-15 of the others', within tiles, between them and between the parts of a cut
+    history; groups of equal values; queries of 2^30 on keys of 2^-30 and the other way round; rows of zeros.
+    Values far below the largest one met so far may lose the bits under 2^-33 of it."""
+    rows, lens = [300, 20, 150, 150, 9], [300, 5000, 400, 400, 3100]
+    q, cache, tables, ctx, last = batch(lens, rows, hq, hkv, d, group, bs, 52)
+    kp, vp = pairs_of(cache, d, bs)
+    page = lambda s, at: tables[s, at].long()  # noqa: E731
+    per = 128 // bs  # pages of a key tile
+    used = [tables[s, : -(-n // bs)].long() for s, n in enumerate(lens)]
+    vp[used[0][1::3]] *= 2.0**15  # within every tile
+    vp[used[0][2::3]] *= 2.0**-15
+    for tile in range(0, len(used[1]) // per, 3):  # between tiles, and so between the parts
+        vp[used[1][tile * per : (tile + 1) * per]] *= 2.0**15
+        vp[used[1][(tile + 1) * per : (tile + 2) * per]] *= 2.0**-15
+    vp[used[4][: 8 * per]] *= 2.0**-15  # from small to large
+    vp[used[4][16 * per :]] *= 2.0**15
+    first = torch.tensor(rows).cumsum(0) - torch.tensor(rows)
+    kp[used[2]] *= 2.0**-30
+    q[first[2] : first[2] + 150] *= 2.0**30
+    kp[used[3]] *= 2.0**30
+    q[first[3] : first[3] + 150] *= 2.0**-30
+    vp[page(3, 2), :, :, 0::2] = 0  # scale 0: equal values
+    kp[page(3, 3), :, :, 0::2] = 0
+    q[5] = 0
+    q[first[1] + 3, 0] = 0
+    scale = d**-0.5
+    out = kops.prefill_attention_kv4(q, cache, tables, ctx, last, scale, bs)
+    want, mag = oracle(q, cache, tables, ctx, last, scale, bs)
+    tol = bound(q, cache, tables, ctx, last, scale, bs, want, mag)
+    vals = ref.kv4_cache_values(cache, d, bs)
+    for s in range(len(rows)):
+        top = torch.nan_to_num(vals[used[s], 1]).abs().amax()
+        tol[first[s] : first[s] + rows[s]] += lens[s] * 2.0**-33 * float(top)
+    held_to(out, want, tol)
+    assert kops.check_status() == 0
+
+
+def test_strides_and_far_pages(kops):
+    """q rows out of a wider tensor, a layer's cache out of an interleaved one, pages beyond 4 GiB."""
+    hq, hkv, d, group, bs = 32, 8, 128, 64, 16
+    rows, lens = [70, 5], [200, 2500]
+    q, cache, tables, ctx, last = batch(lens, rows, hq, hkv, d, group, bs, 53)
+    want = kops.prefill_attention_kv4(q, cache, tables, ctx, last, 0.1, bs)
+    wide = torch.full((75, hq * d + 64), math.nan, dtype=torch.bfloat16, device="cuda")
+    wide[:, : hq * d] = q.flatten(1)
+    nb, far = cache.shape[0], (5 << 30) // (2 * cache[0].numel())
+    both = torch.zeros(far + nb, 2, *cache.shape[1:], dtype=torch.uint8, device="cuda")
+    both[far:, 1] = cache
+    tables += far
+    out = kops.prefill_attention_kv4(wide[:, : hq * d].unflatten(1, (hq, d)), both[:, 1], tables, ctx, last, 0.1, bs)
+    assert torch.equal(out, want) and kops.check_status() == 0
+
+
+def test_other_stream(kops):
+    """Calls on two streams at once do not meet: their items are handed out and their parts kept apart."""
+    hq, hkv, d, group, bs = 32, 8, 128, 64, 16
+    q, cache, tables, ctx, last = batch([900, 6000, 300], [500, 30, 1], hq, hkv, d, group, bs, 54)
+    args = (cache, tables, ctx, last)
+    want = kops.prefill_attention_kv4(q, *args, 0.1, bs), kops.prefill_attention_kv4(q, *args, 0.3, bs)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        side = [kops.prefill_attention_kv4(q, *args, 0.3, bs) for _ in range(4)]
+    here = [kops.prefill_attention_kv4(q, *args, 0.1, bs) for _ in range(4)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[0]) for x in here) and all(torch.equal(x, want[1]) for x in side)
+    assert kops.check_status() == 0
+
+
+def test_a_bad_table_entry_is_reported(kops):
+    """Block 0 is read in its place; rows of other sequences do not move."""
+    hq, hkv, d, group, bs = 8, 2, 128, 64, 16
+    q, cache, tables, ctx, last = batch([200, 3000, 90], [64, 20, 90], hq, hkv, d, group, bs, 55)
+    for bad in (cache.shape[0], -1, 2**31 - 1):
+        spoilt, zero = tables.clone(), tables.clone()
+        spoilt[1, 7], zero[1, 7] = bad, 0
+        out = kops.prefill_attention_kv4(q, cache, spoilt, ctx, last, 0.1, bs)
+        assert kops.check_status() == 3
+        assert torch.equal(out, kops.prefill_attention_kv4(q, cache, zero, ctx, last, 0.1, bs))
+        assert kops.check_status() == 0
