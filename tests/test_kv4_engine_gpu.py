@@ -79,3 +79,22 @@ def test_samples_are_their_seeds_own_runs(cuda, kv):
     while twin.has_work():
         twin.step()
     assert twin.request(rid).outputs == twin.request(other).outputs
+
+
+@pytest.mark.parametrize("kv", [None, "int4"])
+@pytest.mark.parametrize("plen", [64, 65, 75])
+def test_forks_of_one_seed_agree(cuda, kv, plen):
+    """Forks that read the common blocks together and their own copy of the last one draw the same from one seed, and
+    others from another."""
+    prompt = [(5 * i + 2) % 500 for i in range(plen)]
+    cfg = lambda: EngineConfig(D128, device="cuda", max_batch=4, max_model_len=512, num_blocks=64, kv_quant=kv)  # noqa: E731
+    eng = Engine(cfg())
+    rid = eng.add_request(prompt, SamplingParams(max_tokens=20))
+    eng.step()
+    draw = lambda seed: SamplingParams(max_tokens=20, temperature=0.8, top_k=30, seed=seed)  # noqa: E731
+    ids = [eng.fork(rid, draw(seed), keep=plen) for seed in (9, 9, 10)]
+    while eng.has_work():
+        eng.step()
+    a, b, c = (eng.request(i).outputs for i in ids)
+    assert len(a) == 20 and a == b and a != c and eng.blocks.free_blocks == 64
+    assert eng.executor.worker.model.ops.check_status() == 0
