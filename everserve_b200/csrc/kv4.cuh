@@ -4,8 +4,10 @@
 // One layer is uint8 [num_blocks, kv_heads, record]. A group is 64 channels, or the whole head, of
 // one row (one token's K or V of one kv head); with mn and mx its smallest and largest value,
 //   scale = bf16((mx - mn) / 15), zero = bf16(mn), code = clamp(rint((x - zero) / scale), 0, 15),
-// and the value held is scale * code + zero. Rounding (scale, zero) to bf16 keeps any finite bf16
-// input in range and costs a row less than 0.07 scale beside the half step of the code itself.
+// and the value held is scale * code + zero. Codes are chosen against the rounded pair, so a value is held within
+// half a scale, or, in a group that lies far from zero against its range, within what rounding the pair moves
+// the group's ends by: 2^-8 (|mn| + mx - mn). A group holding a value that is not finite, or whose range passes
+// fp32's largest number, reads as NaN. The attention kernels take values and queries below 2^90.
 //
 // The record of a (block, kv head) with block size BS, head dim D and NG = D / group:
 //   K codes [BS][D / 2] | V codes [BS][D / 2] | K (scale, zero) [BS][NG][2] | V (scale, zero) [BS][NG][2]

@@ -133,8 +133,9 @@ def paged_attention(q, cache, block_tables, ctx_lens, q_seq, q_pos, scale: float
 # A group is 64 channels, or the whole head, of one row (one token's K or V of one kv head). With mn and
 # mx its smallest and largest value: scale = bf16((mx - mn) / 15), zero = bf16(mn), code =
 # clamp(round((x - zero) / scale), 0, 15), and the value held is scale * code + zero (a group of equal
-# values has scale 0). A group holding a value that is not finite reads as NaN. A record holds the K
-# codes [bs, d / 2], the V codes, the K pairs (scale, zero) [bs, groups, 2] in bf16, the V pairs.
+# values has scale 0). So a value is held within half a scale, or 2^-8 (|mn| + mx - mn) where that is more. A
+# group holding a value that is not finite, or whose range passes fp32's largest number, reads as NaN. A record
+# holds the K codes [bs, d / 2], the V codes, the K pairs (scale, zero) [bs, groups, 2] in bf16, the V pairs.
 
 
 def kv4_cache_shape(num_blocks: int, kv_heads: int, block_size: int, head_dim: int, group: int = 64) -> tuple[int, int, int]:

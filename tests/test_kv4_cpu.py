@@ -132,3 +132,24 @@ def test_a_lost_page_shows():
     lost = torch.cat([torch.arange(2000), torch.arange(2016, n)])
     for got in (attend(k[lost], v[lost]), attend(k.bfloat16().double(), v.bfloat16().double(), True)):
         assert float((got - want).norm() / want.norm()) > 0.0028
+
+
+def test_what_a_group_holds():
+    """A value is held within half a stored scale or, far from zero, within what rounding the pair to bf16 moves the
+    group's ends by: 2^-8 of its smallest value and of its range. A range past fp32's largest number reads as NaN."""
+    g = torch.Generator().manual_seed(7)
+    for offset in (0.0, -1.0, 10.0, 100.0, -3000.0, 1e30):
+        for spread in (1.0, 0.1):
+            x = torch.randn(200, 64, generator=g) * spread * max(1.0, abs(offset) / 100) + offset
+            c, p = ref.kv4_quantize(x, 1)
+            held = ref.kv4_values(c, p.flatten(-2).contiguous().view(torch.uint8)).double()
+            low, high = x.amin(-1, keepdim=True).double(), x.amax(-1, keepdim=True).double()
+            ends = 2.0**-8 * (low.abs() + (high - low))
+            tol = torch.maximum(0.5 * p[..., 0].double(), ends) * (1 + 1e-4) + 2.0**-22 * (high.abs() + low.abs())
+            assert bool(((held - x.double()).abs() <= tol).all())
+    x = torch.zeros(3, 64)
+    x[0, 0], x[0, 1] = 3e38, -3e38
+    x[1, 0], x[1, 1] = 1.6e38, -1.6e38
+    c, p = ref.kv4_quantize(x, 1)
+    y = ref.kv4_values(c, p.flatten(-2).contiguous().view(torch.uint8))
+    assert bool(y[0].isnan().all()) and bool(torch.isfinite(y[1:]).all())
