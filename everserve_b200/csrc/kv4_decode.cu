@@ -24,9 +24,9 @@
 // order. How a history is cut depends on its length alone: a sequence's result does not depend on the batch.
 //
 // Measured: 2 sequences of 126K keys (32 / 8 heads of 128, 289 MB) in 69 us, 4.2 of the copy's 6.5 TB/s; 48 of
-// up to 8K (64 / 8 heads) in 58 us; 64 of 1K in 27 us. Bound by issue: 280 instructions for 16 keys of a kv head,
-// 104 of them masks and shifts on the integer pipe, at 2.3 of 4 a cycle with 16 warps an SM (20 warps spill:
-// 82 us for the first).
+// up to 8K (64 / 8 heads) in 58 us; 64 of 1K in 27 us. Bound by latency and issue: 280 instructions for 16 keys of a
+// kv head, 88 of them masks, shifts and permutes on the integer pipe, at 2.3 of 4 a cycle with 16 warps an SM
+// (20 warps spill: 82 us for the first).
 #include <algorithm>
 #include <atomic>
 

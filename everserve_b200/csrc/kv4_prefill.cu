@@ -28,12 +28,12 @@
 // synchronisation; a warp of each CTA hands items out ahead of their readers. All waits are bounded and end in
 // the status word.
 //
-// Measured (32 / 8 heads of 128): one prompt of 8192 rows in 622-633 us, 870-885 TFLOP/s, half of what cuBLAS
+// Measured (32 / 8 heads of 128): one prompt of 8192 rows in 605-632 us, 870-910 TFLOP/s, half of what cuBLAS
 // reaches.
 // A key tile takes 4,300 cycles where its 32 MMAs need 2,060 and its exponentials 2,050: each query tile's chain
 // S -> softmax -> P -> MMAs is longer than the two tiles' overlap hides, and the conversion's stores and the MMAs
 // share the shared memory's bandwidth. (An eighth of the exponentials as polynomials on the FMA pipe: slower,
-// 654 us; instructions bound the softmax, not the exponential unit.) 16 prompts of 8191 rows in all take 119 us:
+// 654 us; instructions bound the softmax, not the exponential unit.) 16 prompts of 8191 rows in all take 121 us:
 // an item of three key tiles pays as much again for its query, its first conversion and its output. Two more
 // warps that copied the next item's query ahead made that 130 us.
 #include <algorithm>
@@ -70,7 +70,7 @@ ES_DEVICE bool wait_for(uint64_t* bar, uint32_t parity) {
 template <int D>
 struct PreCfg {
   static constexpr int kChunk = kRows * 128;           // one 64-channel chunk of a 128-row operand
-  static constexpr int kTile = (D / 64) * kChunk;      // a bf16 tile of 128 rows
+  static constexpr int kTile = (D / 64) * kChunk;      // an f16 tile of 128 rows
   static constexpr int kSmem = 1024 + 2 * kTile + 2 * 2 * kTile + 256;
 };
 
@@ -108,7 +108,8 @@ struct PreParams {
 // How a sequence of `tiles` row tiles and `keys` key tiles is cut along its keys: the key tiles of an item, and the
 // items that a row tile has at most. Not at all where its row tiles fill the SMs; else into kCutItems items at most, which
 // bounds its parts in the workspace whatever its length (256 rows of a head an item: 34 to 51 MB at head dim 128).
-// (64 rows on 131K keys, 32 / 8 heads of 128: 203 us, without the bound 245; 900 rows on 60K: 1,265 and 1,237; 509 rows on 0-40K keys, 14 / 2 of 64: 106 and 107.)
+// (64 rows on 131K keys, 32 / 8 heads of 128: 203 us, without the bound 245; 900 rows on 60K: 1,265 and 1,237; 509
+// rows on 0-40K keys, 14 / 2 of 64: 106 and 107.)
 struct Cut {
   int chunk, splits;
 };
@@ -239,8 +240,9 @@ ES_DEVICE uint4 values8(uint32_t w, __half2 s, __half2 z) {
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
-// 2^e as a float, e in [-126, 127], and the exponent of a positive number (of its bits), clamped so that the
-// product of a query row's and a key tile's factor stays a normal number
+// 2^e as a float, e in [-126, 127], and the exponent of a positive number (of its bits), clamped so that these
+// factors stay normal numbers, and the product of a query row's and a key tile's does however small they are
+// (a masked score's -infinity times zero would be NaN; large ones meet infinity where their scores pass fp32)
 ES_DEVICE float pre_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 ES_DEVICE int pre_exponent(uint32_t bits) { return min(100, max(-40, (int)(bits >> 23) - 127)); }
 

@@ -310,7 +310,7 @@ ES_DEVICE void tmem_ld16(uint32_t taddr, float* v) {
   for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
 }
 
-// D[tmem] (+)= A[tmem] * B[smem desc]^T: the A rows are the TMEM lanes, its bf16 K elements packed two a
+// D[tmem] (+)= A[tmem] * B[smem desc]^T: the A rows are the TMEM lanes, its 16-bit K elements packed two a
 // column from `a_tmem` on (K = 16: 8 columns).
 ES_DEVICE void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
